@@ -282,6 +282,69 @@ int cda_b200_prefill_clear_status(void);
  * signal so that the waits behind it run out -- the way the tests exercise the give-up path without faulting anything. */
 int cda_b200_prefill_debug(int wait_limit_us, int withhold_first_k_arrive);
 
+/* Attention of the new tokens of every sequence -- the tree of tokens that a drafting model proposed, or a chain -- over the
+ * paged compressed cache, which already holds their own K and V (cda_b200_paged_encode) as each sequence's last q_len slots.
+ * With k_n, v_n the decoded rows of key n, ctx = seq_lens[b] - q_len and row (t, h):
+ *   x_n   = scale * q.k_n;  softcap > 0: softcap * tanh(x_n / softcap);  then + slope_h * (pos_n - pos_t)
+ *   seen  : n < ctx, or n = ctx + j with bit j of tree_mask[t] set (no mask: j <= t); and pos_t - pos_n < window if window > 0
+ *   out   = sum_n softmax(x)_n v_n over the keys seen, lse = log sum_n exp(x_n); a row that sees none: zeros, -inf
+ * The position of a context key is its place, that of a new token ctx + depth, its depth being its place in a chain and
+ * popcount(mask) - 1 (not below 0) in a tree.
+ *   Q, out (T, H_q, 128) fp16, 16-byte aligned; the group H_q / H_kv is at most 64     cu_seqlens_q (B+1)     seq_lens (B)
+ *   tree_mask (T) int64 or null; with a mask max_query_len is at most 64               alibi_slopes (H_q) fp32 or null
+ *   lse (T, H_q) fp32 or null          workspace >= cda_b200_tree_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ *                                      not to be shared by calls that may overlap; its contents need no preparation
+ * Rows of Q behind the last sequence are not written.  A sequence whose lengths do not fit (q_len > seq_len or
+ * max_query_len, seq_len > max_seq_len, rows outside Q) is skipped and reported by cda_b200_kv_status().
+ * No counterpart in the reference: its decode takes one token per sequence (cda/kernels_cuda/wrappers.py:79-124) and its
+ * prefill a causal chunk without score modifiers (cda/kernels_cuda/fa2_cda.py:98-230). */
+size_t cda_b200_tree_attention_workspace_bytes(int H_q, int H_kv, int max_query_len, int device);
+int cda_b200_tree_attention(const void* Q, const void* kv_cache, const int32_t* block_table, const int32_t* cu_seqlens_q,
+                            const int32_t* seq_lens, const float* cb_K, const float* cb_V, const int64_t* tree_mask,
+                            const float* alibi_slopes, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                            int64_t T, int B, int H_q, int H_kv, int block_size, int block_table_stride, int max_query_len,
+                            int max_seq_len, int64_t num_slots, int slot_bytes, int k_bits, int v_bits, float scale,
+                            float softcap, int window, void* stream);
+
+/* Adds to mass[b, h, n] the attention weight that key n of KV head h got from the rows of sequence b:
+ * sum over its new tokens t and the query heads of the group of weights[t] * exp(x_n - lse[t, head]), with x and the rule of
+ * who sees whom as in cda_b200_tree_attention, whose lse it takes (cda_b200_decode_lse's for single tokens).  Rows with
+ * lse = -inf add nothing.  The sum of a key is taken in a fixed order: the same call gives the same bits.
+ *   mass (B, H_kv, mass_stride) fp32, mass_stride >= max_seq_len       weights (T) fp32 or null: 1
+ * No counterpart in the reference. */
+int cda_b200_attention_mass(const void* Q, const void* kv_cache, const int32_t* block_table, const int32_t* cu_seqlens_q,
+                            const int32_t* seq_lens, const float* cb_K, const int64_t* tree_mask, const float* alibi_slopes,
+                            const float* lse, const float* weights, float* mass, int64_t mass_stride, int64_t T, int B, int H_q,
+                            int H_kv, int block_size, int block_table_stride, int max_query_len, int max_seq_len,
+                            int64_t num_slots, int slot_bytes, int k_bits, int v_bits, float scale, float softcap, int window,
+                            void* stream);
+
+/* Which `budget` keys of every (sequence, KV head) to keep: the first `sink`, the last `recent`, and of the others those with
+ * the largest mass, ties to the lower index (NaN ranks as minus infinity).  keep (B, H_kv, budget) int32 in ascending order,
+ * -1 behind the end of a sequence of fewer keys; new_lens (B) int32 = min(seq_lens, budget).  sink + recent <= budget.
+ *   mass (B, H_kv, mass_stride) fp32; a sequence longer than mass_stride is cut to it and reported (cda_b200_kv_status)
+ * No counterpart in the reference. */
+int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, int32_t* keep, int32_t* new_lens, int B, int H_kv,
+                         int64_t mass_stride, int budget, int sink, int recent, void* stream);
+
+/* Moves slots inside every sequence, in place: the slot of token keep[b, h, i] goes to token start[b] + i (start null: 0).
+ * Every entry must satisfy start[b] + i <= keep < seq_lens[b]; a negative one leaves its destination as it is, one that
+ * breaks the rule is skipped and reported (cda_b200_kv_status).  keep (B, keep_heads, K) int32, keep_heads = H_kv or 1 (one
+ * list for all heads).  With `mass` (B, H_kv, mass_stride) the weights move along: a destination gets its key's weight (0
+ * without a valid entry), and those from start + K to the end of the sequence become 0.  The pages that a sequence writes to
+ * must be its own: a page that two block tables share is moved for both.  Slots behind the moved ones keep their bytes.
+ * No counterpart in the reference. */
+int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table, const int32_t* seq_lens, const int32_t* keep,
+                           const int32_t* start, float* mass, int64_t mass_stride, int B, int H_kv, int K, int keep_heads,
+                           int block_size, int block_table_stride, int64_t num_slots, int slot_bytes, void* stream);
+
+/* What the four calls above saw on the current device since the last clear (sticky bits; synchronises the device):
+ * bit 0 (1) a block-table entry was outside the cache (the attention calls read block 0 instead, the compaction skips the
+ * slot);  bit 2 (4) a bounded wait gave up and rows were left unwritten;  bit 3 (8) lengths that do not fit the call;
+ * bit 4 (16) a refused entry of a keep list or a negative start.  Negative status on a CUDA error. */
+int cda_b200_kv_status(void);
+int cda_b200_kv_clear_status(void);
+
 #ifdef __cplusplus
 }
 #endif

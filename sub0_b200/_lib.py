@@ -59,6 +59,15 @@ PROTOTYPES = {
     "cda_b200_prefill_clear_status": (_i, []),
     "cda_b200_prefill_debug": (_i, [_i, _i]),
     "cda_b200_dequantize_rows": (_i, [_p, _p, _p, _p, _i64, _i, _p]),
+    "cda_b200_tree_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "cda_b200_tree_attention": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i, _i, _i, _i, _i, _i, _i,
+                                     _i64, _i, _i, _i, _f, _f, _i, _p]),
+    "cda_b200_attention_mass": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _i, _i, _i, _i64,
+                                     _i, _i, _i, _f, _f, _i, _p]),
+    "cda_b200_select_keys": (_i, [_p, _p, _p, _p, _i, _i, _i64, _i, _i, _i, _p]),
+    "cda_b200_compact_cache": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _i64, _i, _p]),
+    "cda_b200_kv_status": (_i, []),
+    "cda_b200_kv_clear_status": (_i, []),
 }
 
 

@@ -1,0 +1,227 @@
+// Attention of drafted tokens over the compressed paged cache (tree_attention), and the weight its queries give to every
+// cached key (attention_mass).
+//
+// With k_n, v_n the decoded rows fp16(level * norm) of key n in the rotated frame, q_r the rotated query of row r = (token t,
+// query head h) and ctx = seq_len - q_len:
+//   x_rn  = scale * q_r.k_n,   capped: softcap * tanh(x_rn / softcap),   plus slope_h * (pos_n - pos_t)
+//   sees  = n < ctx or bit (n - ctx) of tree_mask[t] (chain: n <= ctx + t), and pos_t - pos_n < window
+//   lse_r = log sum_n exp(x_rn)      out_r = H (sum_n exp(x_rn - lse_r) v_n)      mass_n += sum_r weight_t exp(x_rn - lse_r)
+// pos of a context key is its place, pos of a new token ctx + depth.  A row that sees no key gives zeros and lse -inf.
+#include "attend.cuh"
+
+#include <cmath>
+
+namespace cda {
+
+__device__ int g_tree_status = 0;
+
+// Four consecutive coordinates 4 * lane .. of one side of a slot, as the stored fp16 values.
+__device__ __forceinline__ void decode4(const uint8_t* codes, int bits, const float* cb, float norm, int lane, float (&v)[4]) {
+  int c[4];
+  if (bits == 4) {
+    const uint8_t a = codes[2 * lane], b = codes[2 * lane + 1];
+    c[0] = a >> 4; c[1] = a & 15; c[2] = b >> 4; c[3] = b & 15;
+  } else {
+    const uint8_t a = codes[lane];
+    c[0] = a >> 6; c[1] = (a >> 4) & 3; c[2] = (a >> 2) & 3; c[3] = a & 3;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = round_to_half(cb[c[i]] * norm);
+}
+
+__device__ __forceinline__ const uint8_t* slot_of(const AttendParams& p, int b, int n, int head, bool& bad) {
+  int blk = p.block_table[static_cast<int64_t>(b) * p.bt_stride + n / p.block_size];
+  if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) { bad = true; blk = 0; }
+  return p.cache + ((static_cast<int64_t>(blk) * p.block_size + n % p.block_size) * p.H_kv + head) * p.slot_bytes;
+}
+
+__device__ __forceinline__ int sequence_of(const AttendParams& p, int64_t token) {
+  int lo = 0, hi = p.B - 1;                       // last b with cu_q[b] <= token
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.cu_q[mid] <= token) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Whether token t of the sequence sees key n, and the bias of the pair.
+__device__ __forceinline__ bool sees(const AttendParams& p, const SequenceView& s, int t, int n, float slope, float& bias) {
+  const int ctx = s.seq_len - s.q_len;
+  const int pos_q = ctx + depth_of(p, s.q_begin, t), pos_k = n < ctx ? n : ctx + depth_of(p, s.q_begin, n - ctx);
+  bias = slope * static_cast<float>(pos_k - pos_q);
+  if (p.window > 0 && pos_q - pos_k >= p.window) return false;
+  if (n < ctx) return true;
+  return p.tree_mask ? (static_cast<unsigned long long>(p.tree_mask[s.q_begin + t]) >> (n - ctx)) & 1ull : n - ctx <= t;
+}
+
+// One warp per (token, query head), one key at a time, everything in fp32.
+__global__ void __launch_bounds__(32) tree_simple_kernel(const AttendParams p) {
+  const int lane = threadIdx.x, hq = blockIdx.x, head = hq / p.group;
+  const int64_t token = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
+  if (token >= p.T) return;
+  const int b = sequence_of(p, token);
+  const SequenceView s = sequence_view(p, b);
+  if (s.bad && lane == 0) atomicOr(&g_tree_status, kStatusLengths);
+  const int t = static_cast<int>(token) - s.q_begin;
+  if (t < 0 || t >= s.q_len) return;
+  float q[4];
+  load_half4(p.q + (token * p.H_q + hq) * kHeadDim + 4 * lane, q);
+  fht128_warp(q, lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] *= kRsqrtD * p.scale;
+  const float slope = p.slopes ? p.slopes[hq] : 0.f, inv_cap = p.softcap > 0.f ? 1.0f / p.softcap : 0.f;
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  bool bad = false;
+  for (int n = 0; n < s.seq_len; ++n) {
+    float bias;
+    if (!sees(p, s, t, n, slope, bias)) continue;
+    const uint8_t* slot = slot_of(p, b, n, head, bad);
+    const float* norms = reinterpret_cast<const float*>(slot + 16 * (p.k_bits + p.v_bits));
+    float k[4], v[4];
+    decode4(slot, p.k_bits, p.cb_k, norms[0], lane, k);
+    decode4(slot + 16 * p.k_bits, p.v_bits, p.cb_v, norms[1], lane, v);
+    float x = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
+    if (p.softcap > 0.f) x = soft_cap(x, p.softcap, inv_cap);
+    x += bias;
+    const float mn = fmaxf(m, x), a = expf(m - mn), w = expf(x - mn);
+    l = l * a + w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = o[i] * a + w * v[i];
+    m = mn;
+  }
+  if (bad && lane == 0) atomicOr(&g_tree_status, kStatusBadBlock);
+  const float inv = l > 0.f ? kRsqrtD / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] *= inv;
+  fht128_warp(o, lane);
+  *reinterpret_cast<uint2*>(p.out + (token * p.H_q + hq) * kHeadDim + 4 * lane) = pack_half4(o);
+  if (p.lse_out && lane == 0) p.lse_out[token * p.H_q + hq] = l > 0.f ? m + logf(l) : -INFINITY;
+}
+
+// One warp per (sequence, KV head, key): the rows one after another.  The key is rotated back once, so that the raw query
+// rows can be used as they are.
+__global__ void __launch_bounds__(256) mass_simple_kernel(const AttendParams p) {
+  const int lane = threadIdx.x & 31, head = blockIdx.y, b = blockIdx.z;
+  const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const SequenceView s = sequence_view(p, b);
+  if (s.bad && threadIdx.x == 0 && blockIdx.x == 0 && head == 0) atomicOr(&g_tree_status, kStatusLengths);
+  if (s.q_len == 0 || n >= s.seq_len) return;
+  bool bad = false;
+  const uint8_t* slot = slot_of(p, b, n, head, bad);
+  if (bad && lane == 0) atomicOr(&g_tree_status, kStatusBadBlock);
+  float k[4];
+  decode4(slot, p.k_bits, p.cb_k, *reinterpret_cast<const float*>(slot + 16 * (p.k_bits + p.v_bits)), lane, k);
+  fht128_warp(k, lane);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k[i] *= kRsqrtD * p.scale;
+  const float inv_cap = p.softcap > 0.f ? 1.0f / p.softcap : 0.f;
+  float sum = 0.f;
+  for (int r = 0; r < s.q_len * p.group; ++r) {
+    const int t = r / p.group, hq = head * p.group + r % p.group;
+    const int64_t row = static_cast<int64_t>(s.q_begin + t) * p.H_q + hq;
+    const float z = p.lse[row], w = p.weights ? p.weights[s.q_begin + t] : 1.0f;
+    float bias;
+    if (!sees(p, s, t, n, p.slopes ? p.slopes[hq] : 0.f, bias) || z == -INFINITY || w == 0.f) continue;
+    float q[4];
+    load_half4(p.q + row * kHeadDim + 4 * lane, q);
+    float x = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
+    if (p.softcap > 0.f) x = soft_cap(x, p.softcap, inv_cap);
+    sum += w * expf(x + bias - z);
+  }
+  if (lane == 0) p.mass[(static_cast<int64_t>(b) * p.H_kv + head) * p.mass_stride + n] += sum;
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------
+static int fill_params(AttendParams& p, const char* what, const void* Q, const void* kv_cache, const int32_t* block_table,
+                       const int32_t* cu_q, const int32_t* seq_lens, const float* cb_K, const int64_t* tree_mask,
+                       const float* slopes, int64_t T, int B, int H_q, int H_kv, int block_size, int bt_stride, int max_q,
+                       int max_n, int64_t num_slots, int slot_bytes, int k_bits, int v_bits, float scale, float softcap, int window) {
+  if (T < 0 || B < 0 || H_q <= 0 || H_kv <= 0 || max_q < 0 || max_n < 0 || num_slots < 0 || window < 0)
+    return fail(CDA_ERR_BAD_ARG, "%s: negative size", what);
+  if (!(softcap >= 0.f) || std::isinf(softcap) || !std::isfinite(scale)) return fail(CDA_ERR_BAD_ARG, "%s: scale and softcap must be finite, softcap not negative", what);
+  if (!bits_ok(k_bits) || !bits_ok(v_bits)) return fail(CDA_ERR_UNSUPPORTED, "%s: bits must be 2 or 4", what);
+  if (H_q % H_kv) return fail(CDA_ERR_BAD_SHAPE, "%s: H_q=%d is not a multiple of H_kv=%d", what, H_q, H_kv);
+  if (H_q / H_kv > 64) return fail(CDA_ERR_UNSUPPORTED, "%s: GQA group %d > 64", what, H_q / H_kv);
+  if (slot_bytes != slot_bytes_for(k_bits, v_bits)) return fail(CDA_ERR_BAD_SHAPE, "%s: slot width %d does not fit k%dv%d", what, slot_bytes, k_bits, v_bits);
+  if (block_size <= 0 || block_size % 16) return fail(CDA_ERR_BAD_SHAPE, "%s: block_size=%d is not a multiple of 16", what, block_size);
+  if (static_cast<int64_t>(bt_stride) * block_size < max_n) return fail(CDA_ERR_BAD_SHAPE, "%s: block table row shorter than max_seq_len", what);
+  if (tree_mask && max_q > 64) return fail(CDA_ERR_UNSUPPORTED, "%s: a tree has at most 64 tokens, max_query_len is %d", what, max_q);
+  if (num_slots / block_size > 0x7fffffffll) return fail(CDA_ERR_N_TOO_LARGE, "%s: too many slots", what);
+  if (B == 0 || T == 0 || max_q == 0 || max_n == 0) return 1;
+  if (num_slots < block_size) return fail(CDA_ERR_BAD_SHAPE, "%s: the cache holds no block", what);
+  if (!Q || !kv_cache || !block_table || !cu_q || !seq_lens || !cb_K) return fail(CDA_ERR_BAD_ARG, "%s: null pointer", what);
+  if (!aligned16(Q) || !aligned16(kv_cache)) return fail(CDA_ERR_BAD_ALIGN, "%s: Q and cache must be 16-byte aligned", what);
+  p.q = static_cast<const __half*>(Q);
+  p.cache = static_cast<const uint8_t*>(kv_cache);
+  p.block_table = block_table; p.cu_q = cu_q; p.seq_lens = seq_lens; p.cb_k = cb_K; p.tree_mask = tree_mask; p.slopes = slopes;
+  p.T = T; p.B = B; p.H_q = H_q; p.H_kv = H_kv; p.group = H_q / H_kv; p.block_size = block_size; p.bt_stride = bt_stride;
+  p.bs_shift = -1;
+  for (int sft = 4; sft < 31; ++sft) if ((1 << sft) == block_size) p.bs_shift = sft;
+  p.num_blocks = static_cast<int>(num_slots / block_size);
+  p.max_q = max_q; p.max_n = max_n; p.k_bits = k_bits; p.v_bits = v_bits; p.slot_bytes = slot_bytes;
+  p.scale = scale; p.softcap = softcap; p.window = window;
+  return CDA_OK;
+}
+
+}  // namespace cda
+
+using namespace cda;
+
+extern "C" size_t cda_b200_tree_attention_workspace_bytes(int H_q, int H_kv, int max_query_len, int device) {
+  (void)H_q; (void)H_kv; (void)max_query_len; (void)device;
+  return 256;
+}
+
+extern "C" int cda_b200_tree_attention(const void* Q, const void* kv_cache, const int32_t* block_table, const int32_t* cu_seqlens_q,
+                                       const int32_t* seq_lens, const float* cb_K, const float* cb_V, const int64_t* tree_mask,
+                                       const float* alibi_slopes, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                       int64_t T, int B, int H_q, int H_kv, int block_size, int block_table_stride, int max_query_len,
+                                       int max_seq_len, int64_t num_slots, int slot_bytes, int k_bits, int v_bits, float scale,
+                                       float softcap, int window, void* stream) {
+  AttendParams p{};
+  const int rc = fill_params(p, "tree_attention", Q, kv_cache, block_table, cu_seqlens_q, seq_lens, cb_K, tree_mask, alibi_slopes, T, B,
+                             H_q, H_kv, block_size, block_table_stride, max_query_len, max_seq_len, num_slots, slot_bytes, k_bits,
+                             v_bits, scale, softcap, window);
+  if (rc == 1) return CDA_OK;
+  if (rc != CDA_OK) return rc;
+  if (!cb_V || !out) return fail(CDA_ERR_BAD_ARG, "tree_attention: null pointer");
+  if (!aligned16(out)) return fail(CDA_ERR_BAD_ALIGN, "tree_attention: out must be 16-byte aligned");
+  if (workspace_bytes < cda_b200_tree_attention_workspace_bytes(H_q, H_kv, max_query_len, -1) || !workspace)
+    return fail(CDA_ERR_WORKSPACE, "tree_attention: workspace of %zu bytes, need %zu", workspace_bytes,
+                cda_b200_tree_attention_workspace_bytes(H_q, H_kv, max_query_len, -1));
+  if (!aligned16(workspace)) return fail(CDA_ERR_BAD_ALIGN, "tree_attention: workspace must be 16-byte aligned");
+  p.cb_v = cb_V; p.out = static_cast<__half*>(out); p.lse_out = lse;
+  const int64_t gy = T < 32768 ? T : 32768;
+  const int64_t gz = (T + gy - 1) / gy;
+  if (gz > 65535) return fail(CDA_ERR_N_TOO_LARGE, "tree_attention: %lld tokens", static_cast<long long>(T));
+  tree_simple_kernel<<<dim3(H_q, static_cast<unsigned>(gy), static_cast<unsigned>(gz)), 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return check_launch("tree_attention");
+}
+
+extern "C" int cda_b200_attention_mass(const void* Q, const void* kv_cache, const int32_t* block_table, const int32_t* cu_seqlens_q,
+                                       const int32_t* seq_lens, const float* cb_K, const int64_t* tree_mask, const float* alibi_slopes,
+                                       const float* lse, const float* weights, float* mass, int64_t mass_stride, int64_t T, int B, int H_q,
+                                       int H_kv, int block_size, int block_table_stride, int max_query_len, int max_seq_len,
+                                       int64_t num_slots, int slot_bytes, int k_bits, int v_bits, float scale, float softcap, int window,
+                                       void* stream) {
+  AttendParams p{};
+  const int rc = fill_params(p, "attention_mass", Q, kv_cache, block_table, cu_seqlens_q, seq_lens, cb_K, tree_mask, alibi_slopes, T, B,
+                             H_q, H_kv, block_size, block_table_stride, max_query_len, max_seq_len, num_slots, slot_bytes, k_bits,
+                             v_bits, scale, softcap, window);
+  if (rc == 1) return CDA_OK;
+  if (rc != CDA_OK) return rc;
+  if (!lse || !mass) return fail(CDA_ERR_BAD_ARG, "attention_mass: null pointer");
+  if (mass_stride < max_seq_len) return fail(CDA_ERR_BAD_SHAPE, "attention_mass: rows of %lld weights, max_seq_len is %d", static_cast<long long>(mass_stride), max_seq_len);
+  if (H_kv > 65535 || B > 65535) return fail(CDA_ERR_N_TOO_LARGE, "attention_mass: B %d or H_kv %d exceeds the grid limits", B, H_kv);
+  p.lse = lse; p.weights = weights; p.mass = mass; p.mass_stride = mass_stride;
+  mass_simple_kernel<<<dim3((max_seq_len + 7) / 8, H_kv, B), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return check_launch("attention_mass");
+}
+
+namespace cda {
+int tree_status(bool clear, int* value) {
+  const int zero = 0;
+  const cudaError_t e = clear ? cudaMemcpyToSymbol(g_tree_status, &zero, sizeof(int)) : cudaMemcpyFromSymbol(value, g_tree_status, sizeof(int));
+  return e == cudaSuccess ? CDA_OK : check_launch("kv_status");
+}
+}  // namespace cda

@@ -405,3 +405,189 @@ def varlen_fwd_hadamard(Q: Tensor, k_rot: Tensor, v_rot: Tensor, output: Tensor,
     check(fn(Qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), output.data_ptr(), cq.data_ptr(), ck.data_ptr(), su.data_ptr(),
              Q.shape[0], cq.numel() - 1, Q.shape[1], k_rot.shape[1], int(max_query_len), int(max_seq_len), float(scale),
              _stream(Q.device)))
+
+
+# ---- drafted tokens, attention weights, eviction ------------------------------------------------------------------------
+
+def _same_device(dev: torch.device, **tensors: Optional[Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _cuda(t, name)
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the call on {dev}")
+
+
+class _AttendArgs:
+    __slots__ = ("Q", "cache", "bt", "cu", "sl", "cbk", "mask", "slopes", "kb", "vb", "head", "tail", "keep", "dev")
+
+
+def _attend_args(Q, kv_cache, block_table, seq_lens, cb_K, k_bits, v_bits, block_size, cu_seqlens_q, max_query_len, max_seq_len, tree_mask,
+                 scale, softcap, alibi_slopes, window) -> _AttendArgs:
+    """The arguments that :func:`tree_attention` and :func:`attention_mass` share, checked; ``head`` and ``tail`` are the
+    shape and rule arguments of both C entry points."""
+    a = _AttendArgs()
+    _cuda(Q, "Q", torch.float16)
+    if Q.dim() != 3 or Q.shape[-1] != HEAD_DIM:
+        raise ValueError("Q must be (T, H_q, 128)")
+    a.dev = Q.device
+    _same_device(a.dev, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, cu_seqlens_q=cu_seqlens_q,
+                 tree_mask=tree_mask, alibi_slopes=alibi_slopes)
+    a.Q, a.cache = Q.contiguous(), _flat_cache(kv_cache)
+    a.bt, a.sl, a.cu = (_i32(t).contiguous() for t in (block_table, seq_lens, cu_seqlens_q))
+    B = a.sl.numel()
+    if a.bt.dim() != 2 or a.bt.shape[0] < B or a.cu.numel() != B + 1:
+        raise ValueError("block_table must be (B, max_blocks), seq_lens (B,) and cu_seqlens_q (B + 1,)")
+    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.numel() != Q.shape[0]):
+        raise ValueError("tree_mask must hold one int64 of ancestor bits per row of Q")
+    if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.numel() != Q.shape[1]):
+        raise ValueError("alibi_slopes must hold one fp32 slope per query head")
+    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
+        raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    if window is not None and window <= 0:
+        raise ValueError(f"window must be positive, got {window}")
+    a.mask = None if tree_mask is None else tree_mask.contiguous()
+    a.slopes = None if alibi_slopes is None else alibi_slopes.contiguous()
+    a.cbk, a.kb, a.vb = _cb(cb_K, a.dev), k_bits, v_bits
+    s = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    a.head = (Q.shape[0], B, Q.shape[1], a.cache.shape[1], int(block_size), a.bt.shape[1], int(max_query_len), int(max_seq_len),
+              a.cache.shape[0], a.cache.shape[2], a.kb, a.vb)
+    a.tail = (s, 0.0 if softcap is None else float(softcap), 0 if window is None else min(int(window), 2 ** 31 - 1))
+    return a
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def tree_attention(Q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, output: Tensor, *, cb_K: Tensor,
+                   cb_V: Tensor, block_size: int, cu_seqlens_q: Tensor, max_query_len: int, max_seq_len: int,
+                   tree_mask: Optional[Tensor] = None, scale: Optional[float] = None, softcap: Optional[float] = None,
+                   alibi_slopes: Optional[Tensor] = None, window: Optional[int] = None, lse: Optional[Tensor] = None,
+                   workspace: Optional[Tensor] = None) -> None:
+    """Attention of every sequence's last tokens -- a drafted tree or a chain -- over the paged cache that already holds their
+    K and V (:func:`paged_encode`).  ``Q``, ``output`` (T, H_q, 128) fp16; sequence b's tokens are rows ``cu_seqlens_q[b]`` to
+    ``cu_seqlens_q[b + 1]`` and its last keys.
+
+    ``tree_mask``: int64 per token, bit j set when it sees the sequence's j-th new token (itself included); at most 64 new
+    tokens per sequence.  Without it the tokens are a causal chain of any length.  ``softcap``: scores become
+    ``softcap * tanh(score / softcap)``.  ``alibi_slopes`` (H_q) fp32: ``slope * (key position - query position)`` is added.
+    ``window``: a key is seen while the query is less than ``window`` positions ahead.  A new token's position is the context
+    plus its depth in the tree.  ``lse``: optional (T, H_q) fp32, log-sum-exp of the row's scores; a row that sees no key gives
+    zeros and -inf.  ``workspace``: uint8 tensor of at least :func:`tree_attention_workspace_bytes`; by default the call takes
+    one from the caching allocator, on its own stream and inside a capture from the graph's pool."""
+    a = _attend_args(Q, kv_cache, block_table, seq_lens, cb_K, _bits_of(cb_K, "cb_K"), _bits_of(cb_V, "cb_V"), block_size,
+                     cu_seqlens_q, max_query_len, max_seq_len, tree_mask, scale, softcap, alibi_slopes, window)
+    _same_device(a.dev, output=output, lse=lse, workspace=workspace)
+    if output.shape != Q.shape or output.dtype != torch.float16 or not output.is_contiguous():
+        raise ValueError("output must be a contiguous fp16 CUDA tensor shaped like Q")
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.numel() != Q.shape[0] * Q.shape[1]):
+        raise ValueError("lse must be a contiguous fp32 CUDA tensor of T * H_q elements")
+    cbv = _cb(cb_V, a.dev)
+    with torch.cuda.device(a.dev):
+        need = tree_attention_workspace_bytes(Q.shape[1], a.cache.shape[1], int(max_query_len))
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=a.dev)
+        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
+        check(lib.cda_b200_tree_attention(a.Q.data_ptr(), a.cache.data_ptr(), a.bt.data_ptr(), a.cu.data_ptr(), a.sl.data_ptr(),
+                                          a.cbk.data_ptr(), cbv.data_ptr(), _ptr(a.mask), _ptr(a.slopes), output.data_ptr(),
+                                          _ptr(lse), workspace.data_ptr(), workspace.numel(), *a.head, *a.tail, _stream(a.dev)))
+
+
+def tree_attention_workspace_bytes(H_q: int, H_kv: int, max_query_len: int, device: int = -1) -> int:
+    return int(lib.cda_b200_tree_attention_workspace_bytes(H_q, H_kv, max_query_len, device))
+
+
+def attention_mass(Q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, lse: Tensor, mass: Tensor, *,
+                   cb_K: Tensor, block_size: int, cu_seqlens_q: Tensor, max_query_len: int, max_seq_len: int,
+                   tree_mask: Optional[Tensor] = None, scale: Optional[float] = None, softcap: Optional[float] = None,
+                   alibi_slopes: Optional[Tensor] = None, window: Optional[int] = None, weights: Optional[Tensor] = None) -> None:
+    """Adds the attention weight that every cached key gets from the rows of ``Q`` to ``mass`` (B, H_kv, M >= max_seq_len)
+    fp32: the sum over a sequence's tokens and a KV head's query heads of ``weights[token] * exp(score - lse)``.  ``lse`` (T,
+    H_q) fp32 is what :func:`tree_attention` (or :func:`decode` for single tokens) wrote for the same call, and the other
+    arguments are that call's.  ``weights``: optional (T,) fp32, e.g. 1 for accepted drafts and 0 for the others."""
+    kb = _bits_of(cb_K, "cb_K")
+    vb = (_flat_cache(_cuda(kv_cache, "kv_cache")).shape[2] - 16) // 16 - kb
+    a = _attend_args(Q, kv_cache, block_table, seq_lens, cb_K, kb, vb, block_size, cu_seqlens_q, max_query_len, max_seq_len,
+                     tree_mask, scale, softcap, alibi_slopes, window)
+    _same_device(a.dev, lse=lse, mass=mass, weights=weights)
+    if lse.dtype != torch.float32 or not lse.is_contiguous() or lse.numel() != Q.shape[0] * Q.shape[1]:
+        raise ValueError("lse must be a contiguous fp32 CUDA tensor of T * H_q elements")
+    if mass.dtype != torch.float32 or not mass.is_contiguous() or mass.dim() != 3 or mass.shape[:2] != (a.sl.numel(), a.cache.shape[1]):
+        raise ValueError("mass must be a contiguous fp32 CUDA tensor (B, H_kv, M)")
+    if weights is not None and (weights.dtype != torch.float32 or not weights.is_contiguous() or weights.numel() != Q.shape[0]):
+        raise ValueError("weights must be a contiguous fp32 CUDA tensor with one element per row of Q")
+    with torch.cuda.device(a.dev):
+        check(lib.cda_b200_attention_mass(a.Q.data_ptr(), a.cache.data_ptr(), a.bt.data_ptr(), a.cu.data_ptr(), a.sl.data_ptr(),
+                                          a.cbk.data_ptr(), _ptr(a.mask), _ptr(a.slopes), lse.data_ptr(), _ptr(weights),
+                                          mass.data_ptr(), mass.shape[2], *a.head, *a.tail, _stream(a.dev)))
+
+
+def select_keys(mass: Tensor, seq_lens: Tensor, budget: int, *, sink: int = 0, recent: int = 0):
+    """The ``budget`` keys of every (sequence, KV head) worth keeping: the first ``sink``, the last ``recent`` and of the others
+    those with the largest ``mass`` (B, H_kv, M), ties to the lower index, NaN as minus infinity.  Returns ``keep`` (B, H_kv,
+    budget) int32, ascending, -1 behind a shorter sequence's end, and ``new_lens`` (B,) int32 = min(seq_lens, budget)."""
+    _cuda(mass, "mass", torch.float32)
+    if mass.dim() != 3 or not mass.is_contiguous():
+        raise ValueError("mass must be a contiguous fp32 CUDA tensor (B, H_kv, M)")
+    _same_device(mass.device, seq_lens=seq_lens)
+    B, H, M = mass.shape
+    sl = _i32(seq_lens).contiguous()
+    if sl.numel() != B:
+        raise ValueError("seq_lens must have one element per sequence of mass")
+    keep = torch.empty(B, H, max(int(budget), 0), dtype=torch.int32, device=mass.device)
+    new_lens = torch.empty(B, dtype=torch.int32, device=mass.device)
+    with torch.cuda.device(mass.device):
+        check(lib.cda_b200_select_keys(mass.data_ptr(), sl.data_ptr(), keep.data_ptr(), new_lens.data_ptr(), B, H, M, int(budget),
+                                       int(sink), int(recent), _stream(mass.device)))
+    return keep, new_lens
+
+
+def compact_cache(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, keep: Tensor, *, block_size: int,
+                  start: Optional[Tensor] = None, mass: Optional[Tensor] = None) -> None:
+    """Moves slots inside every sequence, in place: token ``keep[b, h, i]`` goes to token ``start[b] + i`` (0 without
+    ``start``).  ``keep`` (B, H_kv or 1, K) int32; every entry satisfies ``start[b] + i <= keep < seq_lens[b]`` or is negative,
+    which leaves its destination as it is.  After :func:`select_keys` this shortens the sequences to its ``new_lens``; with
+    ``start`` = the context's length and ``keep`` = the accepted path it moves accepted drafts behind the context.  ``mass``
+    moves along, and becomes 0 from ``start + K`` to the sequence's end.  The pages written to must belong to one sequence."""
+    _cuda(kv_cache, "kv_cache")
+    dev = kv_cache.device
+    _same_device(dev, block_table=block_table, seq_lens=seq_lens, keep=keep, start=start, mass=mass)
+    cache = _flat_cache(kv_cache)
+    bt, sl, kp = _i32(block_table).contiguous(), _i32(seq_lens).contiguous(), _i32(keep).contiguous()
+    st = None if start is None else _i32(start).contiguous()
+    B, H = sl.numel(), cache.shape[1]
+    if bt.dim() != 2 or bt.shape[0] < B or kp.dim() != 3 or kp.shape[0] != B or (st is not None and st.numel() != B):
+        raise ValueError("block_table must be (B, max_blocks), seq_lens and start (B,), keep (B, H_kv or 1, K)")
+    if mass is not None and (mass.dtype != torch.float32 or not mass.is_contiguous() or mass.dim() != 3 or mass.shape[:2] != (B, H)):
+        raise ValueError("mass must be a contiguous fp32 CUDA tensor (B, H_kv, M)")
+    with torch.cuda.device(dev):
+        check(lib.cda_b200_compact_cache(cache.data_ptr(), bt.data_ptr(), sl.data_ptr(), kp.data_ptr(), _ptr(st), _ptr(mass),
+                                         0 if mass is None else mass.shape[2], B, H, kp.shape[2], kp.shape[1], int(block_size),
+                                         bt.shape[1], cache.shape[0], cache.shape[2], _stream(dev)))
+
+
+def evict(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, mass: Tensor, budget: int, *, block_size: int, sink: int = 0,
+          recent: int = 0):
+    """:func:`select_keys` and :func:`compact_cache` in one call: shortens every sequence to its ``budget`` most attended keys
+    per KV head.  Returns ``keep`` (which token each remaining slot held) and the sequences' new lengths."""
+    keep, new_lens = select_keys(mass, seq_lens, budget, sink=sink, recent=recent)
+    compact_cache(kv_cache, block_table, seq_lens, keep, block_size=block_size, mass=mass)
+    return keep, new_lens
+
+
+KV_BAD_BLOCK, KV_WAIT_GAVE_UP, KV_LENGTHS, KV_BAD_KEEP = 1, 4, 8, 16
+
+
+def kv_status() -> int:
+    """Sticky status bits (``KV_*``) that :func:`tree_attention`, :func:`attention_mass`, :func:`select_keys` and
+    :func:`compact_cache` raised on the current device.  Synchronises the device."""
+    rc = lib.cda_b200_kv_status()
+    if rc < 0:
+        check(rc)
+    return rc
+
+
+def kv_clear_status() -> None:
+    check(lib.cda_b200_kv_clear_status())
