@@ -27,6 +27,7 @@ struct AttendParams {
   int64_t mass_stride;
   int64_t T;
   int B, H_q, H_kv, group, block_size, bs_shift, bt_stride, num_blocks, max_q, max_n, k_bits, v_bits, slot_bytes;
+  int row_blocks;                // row blocks per sequence
   float scale, softcap;          // softcap 0: none
   int window;                    // 0: none
 };
@@ -49,19 +50,18 @@ __device__ __forceinline__ int depth_of(const AttendParams& p, int q_begin, int 
   return p.tree_mask ? max(__popcll(static_cast<unsigned long long>(p.tree_mask[q_begin + t])) - 1, 0) : t;
 }
 
-// cap * tanh(x / cap).  tanh.approx is off by up to 2^-11, which on a score of 50 is 0.02 and on its probability 2 %, so:
-// below 0.55 the odd Taylor series to x^15 (truncation below 1e-8 of the value), above it 1 - 2 / (e^2x + 1), where the
-// two approximate instructions leave less than 2^-22.
-__device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap) {
-  const float x = s * inv_cap, ax = fabsf(x), x2 = x * x;
-  float t = 2.0f / 15.0f;
-  t = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -929569.0f / 638512875.0f, 21844.0f / 6081075.0f), -1382.0f / 155925.0f), 62.0f / 2835.0f), -17.0f / 315.0f), t);
+// tanh for capped scores.  tanh.approx is off by up to 2^-11, which on a score near a cap of 50 is 0.02 and on its
+// probability 2 %, so: below 0.55 the odd Taylor series to x^15 (truncation below 5e-8 of the value), above it 1 - 2 / (e^2x +
+// 1), where the two approximate instructions leave less than 2^-22.
+__device__ __forceinline__ float soft_tanh(float x) {
+  const float ax = fabsf(x), x2 = x * x;
+  float t = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -929569.0f / 638512875.0f, 21844.0f / 6081075.0f), -1382.0f / 155925.0f), 62.0f / 2835.0f), -17.0f / 315.0f), 2.0f / 15.0f);
   t = x * fmaf(x2, fmaf(x2, t, -1.0f / 3.0f), 1.0f);
   if (ax >= 0.55f) {
     const float e = fast_exp2(2.0f * kLog2e * fminf(ax, 20.0f));
     t = copysignf(1.0f - __fdividef(2.0f, e + 1.0f), x);
   }
-  return cap * t;
+  return t;
 }
 
 }  // namespace cda

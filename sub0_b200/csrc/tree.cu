@@ -9,11 +9,15 @@
 // pos of a context key is its place, pos of a new token ctx + depth.  A row that sees no key gives zeros and lse -inf.
 #include "attend.cuh"
 
+namespace cda {
+__device__ int g_tree_status = 0;
+}
+
+#include "tree_umma.cuh"
+
 #include <cmath>
 
 namespace cda {
-
-__device__ int g_tree_status = 0;
 
 // Four consecutive coordinates 4 * lane .. of one side of a slot, as the stored fp16 values.
 __device__ __forceinline__ void decode4(const uint8_t* codes, int bits, const float* cb, float norm, int lane, float (&v)[4]) {
@@ -35,15 +39,6 @@ __device__ __forceinline__ const uint8_t* slot_of(const AttendParams& p, int b, 
   return p.cache + ((static_cast<int64_t>(blk) * p.block_size + n % p.block_size) * p.H_kv + head) * p.slot_bytes;
 }
 
-__device__ __forceinline__ int sequence_of(const AttendParams& p, int64_t token) {
-  int lo = 0, hi = p.B - 1;                       // last b with cu_q[b] <= token
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_q[mid] <= token) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
 // Whether token t of the sequence sees key n, and the bias of the pair.
 __device__ __forceinline__ bool sees(const AttendParams& p, const SequenceView& s, int t, int n, float slope, float& bias) {
   const int ctx = s.seq_len - s.q_len;
@@ -52,50 +47,6 @@ __device__ __forceinline__ bool sees(const AttendParams& p, const SequenceView& 
   if (p.window > 0 && pos_q - pos_k >= p.window) return false;
   if (n < ctx) return true;
   return p.tree_mask ? (static_cast<unsigned long long>(p.tree_mask[s.q_begin + t]) >> (n - ctx)) & 1ull : n - ctx <= t;
-}
-
-// One warp per (token, query head), one key at a time, everything in fp32.
-__global__ void __launch_bounds__(32) tree_simple_kernel(const AttendParams p) {
-  const int lane = threadIdx.x, hq = blockIdx.x, head = hq / p.group;
-  const int64_t token = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
-  if (token >= p.T) return;
-  const int b = sequence_of(p, token);
-  const SequenceView s = sequence_view(p, b);
-  if (s.bad && lane == 0) atomicOr(&g_tree_status, kStatusLengths);
-  const int t = static_cast<int>(token) - s.q_begin;
-  if (t < 0 || t >= s.q_len) return;
-  float q[4];
-  load_half4(p.q + (token * p.H_q + hq) * kHeadDim + 4 * lane, q);
-  fht128_warp(q, lane);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] *= kRsqrtD * p.scale;
-  const float slope = p.slopes ? p.slopes[hq] : 0.f, inv_cap = p.softcap > 0.f ? 1.0f / p.softcap : 0.f;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  bool bad = false;
-  for (int n = 0; n < s.seq_len; ++n) {
-    float bias;
-    if (!sees(p, s, t, n, slope, bias)) continue;
-    const uint8_t* slot = slot_of(p, b, n, head, bad);
-    const float* norms = reinterpret_cast<const float*>(slot + 16 * (p.k_bits + p.v_bits));
-    float k[4], v[4];
-    decode4(slot, p.k_bits, p.cb_k, norms[0], lane, k);
-    decode4(slot + 16 * p.k_bits, p.v_bits, p.cb_v, norms[1], lane, v);
-    float x = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-    if (p.softcap > 0.f) x = soft_cap(x, p.softcap, inv_cap);
-    x += bias;
-    const float mn = fmaxf(m, x), a = expf(m - mn), w = expf(x - mn);
-    l = l * a + w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * a + w * v[i];
-    m = mn;
-  }
-  if (bad && lane == 0) atomicOr(&g_tree_status, kStatusBadBlock);
-  const float inv = l > 0.f ? kRsqrtD / l : 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] *= inv;
-  fht128_warp(o, lane);
-  *reinterpret_cast<uint2*>(p.out + (token * p.H_q + hq) * kHeadDim + 4 * lane) = pack_half4(o);
-  if (p.lse_out && lane == 0) p.lse_out[token * p.H_q + hq] = l > 0.f ? m + logf(l) : -INFINITY;
 }
 
 // One warp per (sequence, KV head, key): the rows one after another.  The key is rotated back once, so that the raw query
@@ -125,7 +76,7 @@ __global__ void __launch_bounds__(256) mass_simple_kernel(const AttendParams p) 
     float q[4];
     load_half4(p.q + row * kHeadDim + 4 * lane, q);
     float x = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-    if (p.softcap > 0.f) x = soft_cap(x, p.softcap, inv_cap);
+    if (p.softcap > 0.f) x = p.softcap * soft_tanh(x * inv_cap);
     sum += w * expf(x + bias - z);
   }
   if (lane == 0) p.mass[(static_cast<int64_t>(b) * p.H_kv + head) * p.mass_stride + n] += sum;
@@ -167,9 +118,35 @@ static int fill_params(AttendParams& p, const char* what, const void* Q, const v
 
 using namespace cda;
 
+namespace cda {
+// Rows of a block: the smallest of 16, 32, 64, 128 that holds all rows of the longest chunk, else 128.
+static int rows_per_block(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+static size_t tree_workspace(int NR, int ctas) {
+  return static_cast<size_t>(ctas) * sizeof(tru::Record) + static_cast<size_t>(2) * ctas * NR * (kHeadDim + 2) * sizeof(float);
+}
+
+template <int NR>
+static int launch_tree(AttendParams& p, void* ws, int ctas, cudaStream_t st) {
+  static bool configured[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (cudaFuncSetAttribute(tru::tree_attention_kernel<NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, tru::Cfg<NR>::kSmemBytes) != cudaSuccess)
+      return check_launch("tree_attention: shared memory opt-in");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  tru::tree_attention_kernel<NR><<<ctas, tru::Cfg<NR>::kThreads, tru::Cfg<NR>::kSmemBytes, st>>>(p, ws);
+  const int rc = check_launch("tree_attention");
+  if (rc != CDA_OK) return rc;
+  tru::tree_merge_kernel<NR><<<dim3(ctas, NR / 8), 256, 0, st>>>(p, ws, ctas);
+  return check_launch("tree_attention: merge");
+}
+}  // namespace cda
+
 extern "C" size_t cda_b200_tree_attention_workspace_bytes(int H_q, int H_kv, int max_query_len, int device) {
-  (void)H_q; (void)H_kv; (void)max_query_len; (void)device;
-  return 256;
+  if (H_q <= 0 || H_kv <= 0 || max_query_len < 0) return 0;
+  return tree_workspace(rows_per_block(static_cast<int64_t>(max_query_len) * (H_q / H_kv)), device_sm_count(device));
 }
 
 extern "C" int cda_b200_tree_attention(const void* Q, const void* kv_cache, const int32_t* block_table, const int32_t* cu_seqlens_q,
@@ -191,11 +168,20 @@ extern "C" int cda_b200_tree_attention(const void* Q, const void* kv_cache, cons
                 cda_b200_tree_attention_workspace_bytes(H_q, H_kv, max_query_len, -1));
   if (!aligned16(workspace)) return fail(CDA_ERR_BAD_ALIGN, "tree_attention: workspace must be 16-byte aligned");
   p.cb_v = cb_V; p.out = static_cast<__half*>(out); p.lse_out = lse;
-  const int64_t gy = T < 32768 ? T : 32768;
-  const int64_t gz = (T + gy - 1) / gy;
-  if (gz > 65535) return fail(CDA_ERR_N_TOO_LARGE, "tree_attention: %lld tokens", static_cast<long long>(T));
-  tree_simple_kernel<<<dim3(H_q, static_cast<unsigned>(gy), static_cast<unsigned>(gz)), 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return check_launch("tree_attention");
+  const int ctas = device_sm_count(-1);
+  const int64_t rows = static_cast<int64_t>(max_query_len) * p.group;
+  const int NR = rows_per_block(rows);
+  const int64_t blocks = (rows + NR - 1) / NR;
+  if (blocks * B * H_kv * ((max_seq_len + 127) / 128) > 0x7fffffffll)
+    return fail(CDA_ERR_N_TOO_LARGE, "tree_attention: %d sequences of %d new and %d old tokens are too many tiles for one call", B, max_query_len, max_seq_len);
+  p.row_blocks = static_cast<int>(blocks);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (NR) {
+    case 16: return launch_tree<16>(p, workspace, ctas, st);
+    case 32: return launch_tree<32>(p, workspace, ctas, st);
+    case 64: return launch_tree<64>(p, workspace, ctas, st);
+    default: return launch_tree<128>(p, workspace, ctas, st);
+  }
 }
 
 extern "C" int cda_b200_attention_mass(const void* Q, const void* kv_cache, const int32_t* block_table, const int32_t* cu_seqlens_q,
