@@ -37,6 +37,7 @@
 #include <cuda.h>   // CUtensorMap and the enums of cuTensorMapEncodeTiled (types only: the entry point is looked up at run time)
 
 #include <cstring>
+#include "cache_map.cuh"
 #include "common.cuh"
 
 namespace cda {
@@ -1203,22 +1204,22 @@ static EncodeTiledFn encode_tiled_fn() {
 }
 
 // The cache as a 2-D byte tensor: row = one slot position (all heads, H_kv * slot_bytes bytes), rows = slot positions.
-// A copy box is 16 rows x 160 bytes starting at byte head * slot_bytes: one 16-token group of one head, each slot followed
-// by the first bytes of the next head's slot (or zeros where the box leaves the row), so that a slot lands in a 160-byte
-// cell of the ring stage.
-static int make_cache_map(const char* who, const DecodeCommon& a, CUtensorMap* out) {
+// A copy box is 16 rows x box_bytes starting at byte head * slot_bytes: one 16-token group of one head.  The decode kernel
+// copies 160 bytes a slot: each slot followed by the first bytes of the next head's slot (or zeros where the box leaves the
+// row), so that a slot lands in a 160-byte cell of the ring stage.
+int make_cache_map(const char* who, const void* cache, int H_kv, int slot_bytes, int64_t num_slots, int box_bytes, CUtensorMap* out) {
   const EncodeTiledFn encode = encode_tiled_fn();
   if (encode == nullptr) return fail(CDA_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled is not available from this driver", who);
-  const cuuint64_t row_bytes = static_cast<cuuint64_t>(a.H_kv) * a.slot_bytes;
-  const cuuint64_t dims[2] = {row_bytes, static_cast<cuuint64_t>(a.num_slots)};
+  const cuuint64_t row_bytes = static_cast<cuuint64_t>(H_kv) * slot_bytes;
+  const cuuint64_t dims[2] = {row_bytes, static_cast<cuuint64_t>(num_slots)};
   const cuuint64_t strides[1] = {row_bytes};
-  const cuuint32_t box[2] = {160u, 16u};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes), 16u};
   const cuuint32_t elem[2] = {1u, 1u};
-  const CUresult rc = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(a.cache), dims, strides, box, elem,
+  const CUresult rc = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, elem,
                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) return fail(CDA_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed (%d) for rows of %llu bytes x %lld slots", who,
-                                      static_cast<int>(rc), static_cast<unsigned long long>(row_bytes), static_cast<long long>(a.num_slots));
+                                      static_cast<int>(rc), static_cast<unsigned long long>(row_bytes), static_cast<long long>(num_slots));
   return CDA_OK;
 }
 
@@ -1287,7 +1288,7 @@ static int run_split(const char* who, const DecodeCommon& a, void* workspace, si
   for (int sft = 0; sft < 16; ++sft) if ((1 << sft) == gpb) p.gpb_shift = sft;
   p.smem_bytes = 0;
   CUtensorMap cache_map;
-  int rc = make_cache_map(who, a, &cache_map);
+  int rc = make_cache_map(who, a.cache, a.H_kv, a.slot_bytes, a.num_slots, 160, &cache_map);
   if (rc != CDA_OK) return rc;
   rc = p.group <= 4 ? dispatch_bits<4>(p, pl, cache_map, a.k_bits, a.v_bits, st) : dispatch_bits<8>(p, pl, cache_map, a.k_bits, a.v_bits, st);
   if (rc != CDA_OK) return rc;

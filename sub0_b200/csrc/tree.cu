@@ -97,7 +97,7 @@ static int fill_params(AttendParams& p, const char* what, const void* Q, const v
   if (block_size <= 0 || block_size % 16) return fail(CDA_ERR_BAD_SHAPE, "%s: block_size=%d is not a multiple of 16", what, block_size);
   if (static_cast<int64_t>(bt_stride) * block_size < max_n) return fail(CDA_ERR_BAD_SHAPE, "%s: block table row shorter than max_seq_len", what);
   if (tree_mask && max_q > 64) return fail(CDA_ERR_UNSUPPORTED, "%s: a tree has at most 64 tokens, max_query_len is %d", what, max_q);
-  if (num_slots / block_size > 0x7fffffffll) return fail(CDA_ERR_N_TOO_LARGE, "%s: too many slots", what);
+  if (num_slots > 0x7fffffffll) return fail(CDA_ERR_N_TOO_LARGE, "%s: too many slots", what);
   if (B == 0 || T == 0 || max_q == 0 || max_n == 0) return 1;
   if (num_slots < block_size) return fail(CDA_ERR_BAD_SHAPE, "%s: the cache holds no block", what);
   if (!Q || !kv_cache || !block_table || !cu_q || !seq_lens || !cb_K) return fail(CDA_ERR_BAD_ARG, "%s: null pointer", what);
@@ -127,7 +127,7 @@ static size_t tree_workspace(int NR, int ctas) {
 }
 
 template <int NR>
-static int launch_tree(AttendParams& p, void* ws, int ctas, cudaStream_t st) {
+static int launch_tree(AttendParams& p, void* ws, int ctas, const CUtensorMap& map, cudaStream_t st) {
   static bool configured[64];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -136,7 +136,7 @@ static int launch_tree(AttendParams& p, void* ws, int ctas, cudaStream_t st) {
       return check_launch("tree_attention: shared memory opt-in");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  tru::tree_attention_kernel<NR><<<ctas, tru::Cfg<NR>::kThreads, tru::Cfg<NR>::kSmemBytes, st>>>(p, ws);
+  tru::tree_attention_kernel<NR><<<ctas, tru::Cfg<NR>::kThreads, tru::Cfg<NR>::kSmemBytes, st>>>(p, ws, map);
   const int rc = check_launch("tree_attention");
   if (rc != CDA_OK) return rc;
   tru::tree_merge_kernel<NR><<<dim3(ctas, NR / 8), 256, 0, st>>>(p, ws, ctas);
@@ -175,12 +175,14 @@ extern "C" int cda_b200_tree_attention(const void* Q, const void* kv_cache, cons
   if (blocks * B * H_kv * ((max_seq_len + 127) / 128) > 0x7fffffffll)
     return fail(CDA_ERR_N_TOO_LARGE, "tree_attention: %d sequences of %d new and %d old tokens are too many tiles for one call", B, max_query_len, max_seq_len);
   p.row_blocks = static_cast<int>(blocks);
+  CUtensorMap map;
+  if (const int map_rc = make_cache_map("tree_attention", kv_cache, H_kv, slot_bytes, static_cast<int64_t>(p.num_blocks) * block_size, slot_bytes, &map)) return map_rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (NR) {
-    case 16: return launch_tree<16>(p, workspace, ctas, st);
-    case 32: return launch_tree<32>(p, workspace, ctas, st);
-    case 64: return launch_tree<64>(p, workspace, ctas, st);
-    default: return launch_tree<128>(p, workspace, ctas, st);
+    case 16: return launch_tree<16>(p, workspace, ctas, map, st);
+    case 32: return launch_tree<32>(p, workspace, ctas, map, st);
+    case 64: return launch_tree<64>(p, workspace, ctas, map, st);
+    default: return launch_tree<128>(p, workspace, ctas, map, st);
   }
 }
 

@@ -10,8 +10,9 @@
 // since a lane is a key, the K producers hand their expanded rows to the tensor core through tensor memory, lane by lane,
 // without a pass through shared memory.
 //
-// Warps: softmax (2 or 4 groups of four warps; a thread is a key, a group has NR / groups of the rows), K producers (4), V
-// producers (4; a thread is a key: cache slot -> ring in shared memory by cp.async -> exact fp16 row), one MMA warp.
+// Warps: softmax (2 or 4 groups of four warps; a thread is a key, a group has NR / groups of the rows), K producers and V
+// producers (four each; a thread is a key), one MMA warp, one feeder that brings the slots into a ring in shared memory with
+// tensor-map copies of 16 slots of one head.
 // A CTA walks an equal share of all (sequence, row block, KV head) segments' tiles; a segment that starts and ends in one CTA
 // is finished there, the pieces of the others are merged by tree_merge_kernel.
 //
@@ -20,6 +21,7 @@
 // slow path, which finds the tile's row maxima across lanes and rescales O and the sums.
 #pragma once
 #include "attend.cuh"
+#include "cache_map.cuh"
 #include "expand.cuh"
 #include "umma.cuh"
 
@@ -29,8 +31,8 @@ namespace tru {
 using namespace umma;
 
 constexpr int kKeys = 128, kTileBytes = 32768, kColBlock = 16384;
-constexpr int kCell = 80;                        // one side of one slot in the ring: 64 bytes of codes, 16 with the norms
-constexpr int kStageBytes = 2 * kKeys * kCell;
+constexpr int kStageBytes = kKeys * 144;         // 128 slots side by side; their widths (144, 112, 80) are odd multiples of 16,
+                                                 // so threads that read the same piece of 8 neighbouring slots meet no conflict
 constexpr float kNoRef = 1.0e30f;                // stored negated reference of a row without one: any score exceeds it
 constexpr float kSafe = 14.0f;
 
@@ -41,11 +43,11 @@ struct Cfg {
   static constexpr int kChunk = kCols < 16 ? kCols : 16;
   static constexpr int kChunks = kCols / kChunk;
   static constexpr int kSoftWarps = 4 * kGroups;
-  static constexpr int kWarpK = kSoftWarps, kWarpV = kSoftWarps + 4, kWarpMma = kSoftWarps + 8;
-  static constexpr int kThreads = (kWarpMma + 1) * 32;
+  static constexpr int kWarpK = kSoftWarps, kWarpV = kSoftWarps + 4, kWarpMma = kSoftWarps + 8, kWarpFeed = kWarpMma + 1;
+  static constexpr int kThreads = (kWarpFeed + 1) * 32;
   static constexpr int kPStages = NR == 128 ? 1 : 2;
   static constexpr int kPBytes = kColBlock * (NR == 128 ? 2 : 1);
-  static constexpr int kRing = NR == 128 ? 3 : NR == 64 ? 4 : 5;
+  static constexpr int kRing = NR == 128 ? 3 : NR == 64 ? 5 : 6;
   static constexpr int kTmemCols = NR <= 32 ? 256 : 512;
   static constexpr int kColK = 0, kColS = 128, kColO = 128 + 2 * NR;
   // shared memory (bytes from a 1024-aligned base)
@@ -58,11 +60,11 @@ struct Cfg {
   static constexpr int kOffMax = kOffMask + 8 * NR;               // 4 warps x NR floats
   static constexpr int kOffLevels = kOffMax + 16 * NR;            // 2 x 16 floats
   static constexpr int kOffBar = kOffLevels + 128;                // barriers, TMEM address, wait state, plan
-  static constexpr int kSmemBytes = kOffBar + 256 + 1024;
+  static constexpr int kSmemBytes = kOffBar + 320 + 1024;
   static_assert(kSmemBytes <= 232448, "one CTA's shared memory");
 };
-constexpr int kKFull = 0, kVFull = 2, kSFull = 4, kSEmpty = 6, kPFull = 8, kPvDone = 10, kQFull = 12, kDrained = 13;
-constexpr int kOffTmemAddr = 112, kOffWait = 128, kOffPlan = 160, kOffScan = 192;   // inside kOffBar; scan words share kOffMax
+constexpr int kKFull = 0, kVFull = 2, kSFull = 4, kSEmpty = 6, kPFull = 8, kPvDone = 10, kQFull = 12, kDrained = 13, kRingFull = 14, kRingEmpty = 20;
+constexpr int kOffTmemAddr = 208, kOffWait = 216, kOffPlan = 232, kOffValid = 256;   // inside kOffBar; valid: keys of each ring stage
 
 // ---- shared memory access -----------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -119,13 +121,27 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[N]
   else tmem_st16(addr, v);
 }
 
-// A bounded wait for a barrier phase.  Once a wait of the CTA has given up, every later one returns after one attempt: all
-// roles then run their loops to the end (so nobody is left at a named barrier) without issuing or writing anything.
+// A bounded wait for a barrier phase.  An attempt lets the hardware park the warp for up to kParkNs, so that waiting warps
+// leave the issue slots to the working ones (attempts without the hint, with the timer read between them, cost the
+// working warps three quarters of their speed).  Once a wait of the CTA has given up, every later one returns after one
+// attempt: all roles then run their loops to the end (so nobody is left at a named barrier) without issuing or writing.
+constexpr uint32_t kParkNs = 20000;
+__device__ __forceinline__ bool park_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(kParkNs)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile WaitState* ws) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (park_wait(bar, parity)) return true;
   const unsigned long long t0 = global_timer_ns();
   while (!ws->abort && global_timer_ns() - t0 < ws->limit_ns)
-    if (mbar_try_wait(bar, parity)) return true;
+    if (park_wait(bar, parity)) return true;
   ws->abort = 1;
   return false;
 }
@@ -236,51 +252,21 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int* s_scan, i
   __syncthreads();
 }
 
-// ---- producers ------------------------------------------------------------------------------------------------------------
-// One thread per key.  issue() starts the copies of the walk's next tile into the thread's own ring cells; block ids are read
-// one tile ahead of the slots they address.
-template <int NR>
-struct SlotFeed {
-  Walk<NR> w;
-  Piece q;
-  int tile, end, key, side, bid;
-  bool live, bad;
-  __device__ __forceinline__ int token() const { return min(tile * kKeys + key, q.x.seq_len - 1); }   // keys past the end are masked later
-  __device__ __forceinline__ void fetch_id(const AttendParams& p) {
-    const int n = token();
-    bid = __ldg(p.block_table + static_cast<int64_t>(q.x.b) * p.bt_stride + (p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size));
-  }
-  __device__ __forceinline__ void start(const AttendParams& p) {
-    bad = false;
-    live = w.next(p, q);
-    if (live) { tile = q.tile0; end = q.tile0 + q.n; fetch_id(p); }
-  }
-  __device__ __forceinline__ void issue(const AttendParams& p, uint32_t cell) {
-    if (live) {
-      const int n = token(), in = p.bs_shift >= 0 ? n & (p.block_size - 1) : n % p.block_size;
-      if (static_cast<unsigned>(bid) >= static_cast<unsigned>(p.num_blocks)) { bad = true; bid = 0; }
-      const uint8_t* slot = p.cache + ((static_cast<int64_t>(bid) * p.block_size + in) * p.H_kv + q.head) * p.slot_bytes;
-      const uint8_t* codes = slot + (side ? 16 * p.k_bits : 0);
-      const int bits = side ? p.v_bits : p.k_bits;
-      cp_async16(cell, codes);
-      cp_async16(cell + 16, codes + 16);
-      if (bits == 4) {
-        cp_async16(cell + 32, codes + 32);
-        cp_async16(cell + 48, codes + 48);
-      }
-      cp_async16(cell + 64, slot + 16 * (p.k_bits + p.v_bits));
-      if (++tile == end) {
-        live = w.next(p, q);
-        if (live) { tile = q.tile0; end = q.tile0 + q.n; }
-      }
-      if (live) fetch_id(p);
-    }
-    cp_async_commit();
-  }
-};
+// ---- copies ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// 16 slots of one head (a box of 16 rows x slot_bytes at byte x of row y) -> shared memory; x is head * slot_bytes, a multiple
+// of 16, the destination a multiple of 128.
+__device__ __forceinline__ void copy_group(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+               : "memory");
+}
 
 template <int NR>
-__global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(const AttendParams p, void* ws) {
+__global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(const AttendParams p, void* ws,
+                                                                                   const __grid_constant__ CUtensorMap map) {
   using C = Cfg<NR>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -305,6 +291,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     }
     mbar_init(bar(kQFull), C::kSoftWarps);
     mbar_init(bar(kDrained), 1);
+    for (int i = 0; i < C::kRing; ++i) { mbar_init(bar(kRingFull + i), 1); mbar_init(bar(kRingEmpty + i), 8); }
     wait->abort = 0;
     wait->limit_ns = kWaitLimitNs;
     mbar_init_fence();
@@ -595,96 +582,91 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       }
       group_barrier(group);                                     // the rows' words may be overwritten
     }
-  } else if (warp < C::kWarpV) {
-    // ============ K producers: slot -> exact fp16 row -> tensor memory, lane = key ===========================================
-    const int key = tid - C::kWarpK * 32;
-    const uint32_t cell0 = base + C::kOffRing + key * kCell, lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const float* levels = reinterpret_cast<const float*>(sm + C::kOffLevels);
-    SlotFeed<NR> feed{w};
-    feed.key = key; feed.side = 0;
-    feed.start(p);
-    for (int s = 0; s < C::kRing - 1; ++s) feed.issue(p, cell0 + s * kStageBytes);
-    int stage = 0;
+  } else if (warp < C::kWarpMma) {
+    // ============ producers: slot -> exact fp16 row; K to tensor memory (lane = key), V to shared memory (row = key) ==========
+    const bool is_v = warp >= C::kWarpV;
+    const int key = (warp & 3) * 32 + lane, bits = is_v ? p.v_bits : p.k_bits;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + C::kColK;
+    const uint32_t cell0 = base + C::kOffRing + key * p.slot_bytes, code_at = is_v ? 16 * p.k_bits : 0;
+    const uint32_t norm_at = 16 * (p.k_bits + p.v_bits) + (is_v ? 4 : 0), row = base + C::kOffV;
+    const float* levels = reinterpret_cast<const float*>(sm + C::kOffLevels) + (is_v ? 16 : 0);
+    const int full = is_v ? kVFull : kKFull, freed = is_v ? kPvDone : kSFull;
+    int stage = 0, turn = 0;
 #pragma unroll 1
     for (int i = 0; i < total; ++i) {
-      cp_async_wait<C::kRing - 2>();
+      wait_for(bar(kRingFull + stage), turn, wait);
       const uint32_t cell = cell0 + stage * kStageBytes;
-      uint4 words[4];
-      const float norm = lds_f(cell + 64);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) words[c] = c < 2 || p.k_bits == 4 ? lds128(cell + 16 * c) : make_uint4(0, 0, 0, 0);
-      const int ahead = stage == 0 ? C::kRing - 1 : stage - 1;
-      feed.issue(p, cell0 + ahead * kStageBytes);
-      stage = stage + 1 == C::kRing ? 0 : stage + 1;
-      if (i >= 2) wait_for(bar(kSFull + (i & 1)), ((i - 2) >> 1) & 1, wait);
+      const int valid = *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage);
+      const float norm = key < valid ? lds_f(cell + norm_at) : 0.f;       // keys past the end: zero rows
+      const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
+      if (i >= 2) wait_for(bar(freed + (i & 1)), ((i - 2) >> 1) & 1, wait);
       __syncwarp();
       tc_fence_after_sync();
-      const uint32_t to = lanes + C::kColK + (i & 1) * 64;
-      if (p.k_bits == 4) {
-        const expand::Planes t = expand::make_planes(levels, 4, norm);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[16];
-          expand::quarter4(t, words[c], v);
-          tmem_st16(to + 16 * c, v);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {                                        // 32 coordinates at a time
+        uint32_t v[16];
+        if (bits == 4) {
+          expand::quarter4(t, lds128(cell + code_at + 16 * c), v);
+        } else {
+          const uint2 w = lds64(cell + code_at + 8 * c);
+          expand::quarter2(t, w.x, w.y, v);
         }
-      } else {
-        const expand::Planes t = expand::make_planes(levels, 1, norm);
+        if (is_v) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[16];
-          if (c & 1) expand::quarter2(t, words[c >> 1].z, words[c >> 1].w, v);
-          else expand::quarter2(t, words[c >> 1].x, words[c >> 1].y, v);
-          tmem_st16(to + 16 * c, v);
+          for (int u = 0; u < 4; ++u)
+            sts128(row + (i & 1) * kTileBytes + (c >> 1) * kColBlock + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        } else {
+          tmem_st16(lanes + (i & 1) * 64 + 16 * c, v);
         }
       }
-      tmem_wait_st();
+      if (is_v) fence_async_smem();
+      else tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kKFull + (i & 1)));
-    }
-    cp_async_wait<0>();
-    if (feed.bad) atomicOr(&g_tree_status, kStatusBadBlock);
-  } else if (warp < C::kWarpMma) {
-    // ============ V producers: slot -> exact fp16 row -> shared memory, row = key ============================================
-    const int key = tid - C::kWarpV * 32;
-    const uint32_t cell0 = base + C::kOffRing + kKeys * kCell + key * kCell;
-    const float* levels = reinterpret_cast<const float*>(sm + C::kOffLevels) + 16;
-    SlotFeed<NR> feed{w};
-    feed.key = key; feed.side = 1;
-    feed.start(p);
-    for (int s = 0; s < C::kRing - 1; ++s) feed.issue(p, cell0 + s * kStageBytes);
-    int stage = 0;
-#pragma unroll 1
-    for (int i = 0; i < total; ++i) {
-      cp_async_wait<C::kRing - 2>();
-      const uint32_t cell = cell0 + stage * kStageBytes;
-      uint4 words[4];
-      const float norm = lds_f(cell + 68);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) words[c] = c < 2 || p.v_bits == 4 ? lds128(cell + 16 * c) : make_uint4(0, 0, 0, 0);
-      const int ahead = stage == 0 ? C::kRing - 1 : stage - 1;
-      feed.issue(p, cell0 + ahead * kStageBytes);
-      stage = stage + 1 == C::kRing ? 0 : stage + 1;
-      if (i >= 2) wait_for(bar(kPvDone + (i & 1)), ((i - 2) >> 1) & 1, wait);
-      __syncwarp();
-      const uint32_t to = base + C::kOffV + (i & 1) * kTileBytes;
-      const expand::Planes t = expand::make_planes(levels, p.v_bits == 4 ? 4 : 1, norm);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[16];
-        if (p.v_bits == 4) expand::quarter4(t, words[c], v);
-        else if (c & 1) expand::quarter2(t, words[c >> 1].z, words[c >> 1].w, v);
-        else expand::quarter2(t, words[c >> 1].x, words[c >> 1].y, v);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          sts128(to + (c >> 1) * kColBlock + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+      if (lane == 0) {
+        mbar_arrive(bar(kRingEmpty + stage));
+        mbar_arrive(bar(full + (i & 1)));
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kVFull + (i & 1)));
+      if (++stage == C::kRing) { stage = 0; turn ^= 1; }
     }
-    cp_async_wait<0>();
+  } else if (warp == C::kWarpFeed) {
+    // ============ feeder: one lane per 16-token group of a tile; block ids are read one tile ahead ============================
+    Piece q;
+    bool live = w.next(p, q), bad = false, alive = true;
+    int tile = live ? q.tile0 : 0, stage = 0, turn = 0, issued = 0;
+    auto block_id = [&]() {
+      const int n = min(tile * kKeys + 16 * (lane & 7), q.x.seq_len - 1);
+      return __ldg(p.block_table + static_cast<int64_t>(q.x.b) * p.bt_stride + (p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size));
+    };
+    int id = live ? block_id() : 0;
+#pragma unroll 1
+    while (live && alive) {
+      if (issued >= C::kRing) alive = wait_for(bar(kRingEmpty + stage), turn ^ 1, wait);
+      if (!__all_sync(0xffffffffu, alive)) break;
+      const int left = q.x.seq_len - tile * kKeys, groups = min(8, (left + 15) >> 4), n = tile * kKeys + 16 * lane;
+      if (lane == 0) {
+        *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage) = min(left, kKeys);
+        expect_bytes(bar(kRingFull + stage), groups * 16 * p.slot_bytes);
+      }
+      __syncwarp();
+      if (lane < groups) {
+        if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) { bad = true; id = 0; }
+        const int in = p.bs_shift >= 0 ? n & (p.block_size - 1) : n % p.block_size;
+        copy_group(base + C::kOffRing + stage * kStageBytes + lane * 16 * p.slot_bytes, &map, q.head * p.slot_bytes, id * p.block_size + in, bar(kRingFull + stage));
+      }
+      ++issued;
+      if (++stage == C::kRing) { stage = 0; turn ^= 1; }
+      if (++tile == q.tile0 + q.n) {
+        live = w.next(p, q);
+        if (live) tile = q.tile0;
+      }
+      if (live) id = block_id();
+    }
+    if (bad) atomicOr(&g_tree_status, kStatusBadBlock);
+    // no copy may be in flight when the CTA ends, also after a wait elsewhere gave up
+    const unsigned long long t0 = global_timer_ns();
+    for (int k = max(0, issued - C::kRing); k < issued; ++k)
+      while (!park_wait(bar(kRingFull + k % C::kRing), (k / C::kRing) & 1) && global_timer_ns() - t0 < kWaitLimitNs) { }
   } else if (lane == 0) {
     // ============ MMA issuer =================================================================================================
     constexpr uint32_t idesc_s = instr_desc_f16(kKeys, NR, false, false), idesc_o = instr_desc_f16(kHeadDim, NR, true, true);
