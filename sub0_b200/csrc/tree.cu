@@ -175,6 +175,7 @@ extern "C" int cda_b200_tree_attention(const void* Q, const void* kv_cache, cons
   if (blocks * B * H_kv * ((max_seq_len + 127) / 128) > 0x7fffffffll)
     return fail(CDA_ERR_N_TOO_LARGE, "tree_attention: %d sequences of %d new and %d old tokens are too many tiles for one call", B, max_query_len, max_seq_len);
   p.row_blocks = static_cast<int>(blocks);
+  p.group_magic = static_cast<uint32_t>(((1ull << 32) + p.group - 1) / p.group);
   CUtensorMap map;
   if (const int map_rc = make_cache_map("tree_attention", kv_cache, H_kv, slot_bytes, static_cast<int64_t>(p.num_blocks) * block_size, slot_bytes, &map)) return map_rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

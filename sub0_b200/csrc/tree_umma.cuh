@@ -10,9 +10,9 @@
 // since a lane is a key, the K producers hand their expanded rows to the tensor core through tensor memory, lane by lane,
 // without a pass through shared memory.
 //
-// Warps: softmax (2 or 4 groups of four warps; a thread is a key, a group has NR / groups of the rows), K producers and V
-// producers (four each; a thread is a key), one MMA warp, one feeder that brings the slots into a ring in shared memory with
-// tensor-map copies of 16 slots of one head.
+// Warps: four softmax groups, two K producer groups and one V producer group of four warps each (a thread is a key), two MMA issuers, and a feeder that brings the slots into a ring in shared memory with tensor-map copies of
+// 16 slots of one head.  In a group that waits, one warp polls and the others are parked on a named barrier, where they take no
+// issue slots (27 polling warps spent a third of the kernel's instructions).
 // A CTA walks an equal share of all (sequence, row block, KV head) segments' tiles; a segment that starts and ends in one CTA
 // is finished there, the pieces of the others are merged by tree_merge_kernel.
 //
@@ -33,38 +33,51 @@ using namespace umma;
 constexpr int kKeys = 128, kTileBytes = 32768, kColBlock = 16384;
 constexpr int kStageBytes = kKeys * 144;         // 128 slots side by side; their widths (144, 112, 80) are odd multiples of 16,
                                                  // so threads that read the same piece of 8 neighbouring slots meet no conflict
+constexpr int kCopies = 8;                       // of the value table, one for every four lanes: 8 KB and about two wavefronts a
+constexpr int kRowShift = 5;                     // look-up (32 copies: 32 KB, one wavefront, and one ring stage less)
+constexpr uint32_t kRowMask = 255u << kRowShift; // a table row is 4 * kCopies bytes
 constexpr float kNoRef = 1.0e30f;                // stored negated reference of a row without one: any score exceeds it
 constexpr float kSafe = 14.0f;
+constexpr int kPieceCost = 3;                    // what starting and ending a piece costs, in tiles (the share of a CTA counts it)
 
 template <int NR>
 struct Cfg {
-  static constexpr int kGroups = NR == 128 ? 4 : 2;
-  static constexpr int kCols = NR / kGroups;                     // rows of one softmax group = score columns of one thread
-  static constexpr int kChunk = kCols < 16 ? kCols : 16;
-  static constexpr int kChunks = kCols / kChunk;
-  static constexpr int kSoftWarps = 4 * kGroups;
-  static constexpr int kWarpK = kSoftWarps, kWarpV = kSoftWarps + 4, kWarpMma = kSoftWarps + 8, kWarpFeed = kWarpMma + 1;
-  static constexpr int kThreads = (kWarpFeed + 1) * 32;
-  static constexpr int kPStages = NR == 128 ? 1 : 2;
-  static constexpr int kPBytes = kColBlock * (NR == 128 ? 2 : 1);
-  static constexpr int kRing = NR == 128 ? 3 : NR == 64 ? 5 : 6;
-  static constexpr int kTmemCols = NR <= 32 ? 256 : 512;
-  static constexpr int kColK = 0, kColS = 128, kColO = 128 + 2 * NR;
+  // up to 64 rows: two pairs of groups take tiles in turn (streams), each with its own references, sums and O; 128 rows: all
+  // four share every tile, since two O of 128 columns do not fit the tensor memory
+  static constexpr int kStreams = NR == 128 ? 1 : 2;
+  static constexpr int kCols = NR * kStreams / 4;                // columns of a softmax group
+  static constexpr int kSBuffers = 2 * kStreams, kSShift = kStreams;   // S tiles; log2 of it
+  static constexpr int kBlock = kCols < 16 ? kCols : 16;         // columns worked on at a time
+  static constexpr int kOwn = NR / 4;                            // rows that a group prepares and writes out,
+  static constexpr int kChunk = kOwn < 16 ? kOwn : 16;           // so many at a time
+  static constexpr int kSoftWarps = 16, kProducerWarps = 12;     // four softmax groups; two K groups, one V group
+  static constexpr int kWarpK = kSoftWarps, kWarpV = kWarpK + 8, kWarpS = kWarpV + 4, kWarpO = kWarpS + 1, kWarpFeed = kWarpO + 1;
+  static constexpr int kThreads = (kWarpFeed + 2) * 32;          // the last warp is idle: registers are handed out by four warps
+  // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536)
+  static constexpr int kRegsSoft = 88, kRegsK = 40, kRegsV = 40, kRegsOther = 40;
+  static constexpr int kRing = NR == 128 ? 2 : 4;
+  static constexpr int kTmemCols = 512;                          // tensor memory: two K, the S, one O for each stream
+  static constexpr int kColK = 0, kColS = 128, kColO = kColS + kSBuffers * NR;
   // shared memory (bytes from a 1024-aligned base)
-  static constexpr int kOffV = 0, kOffP = 2 * kTileBytes, kOffQ = kOffP + kPStages * kPBytes, kOffRing = kOffQ + NR * 512;
-  static constexpr int kOffRef = kOffRing + kRing * kStageBytes;  // NR floats: negated references
-  static constexpr int kOffFac = kOffRef + 4 * NR;                // NR floats: factors of a slow path
-  static constexpr int kOffPos = kOffFac + 4 * NR;                // NR ints: positions of the rows
-  static constexpr int kOffSlope = kOffPos + 4 * NR;              // NR floats: slopes x log2 e
-  static constexpr int kOffMask = kOffSlope + 4 * NR;             // NR 64-bit ancestor masks
-  static constexpr int kOffMax = kOffMask + 8 * NR;               // 4 warps x NR floats
-  static constexpr int kOffLevels = kOffMax + 16 * NR;            // 2 x 16 floats
+  static constexpr int kOffV = 0, kOffP = 2 * kTileBytes, kOffQ = kOffP + 2 * kColBlock,   // P: one of 64 rows for each stream, or one of 128
+                        kOffRing = kOffQ + NR * 512;
+  static constexpr int kOffTab = kOffRing + kRing * kStageBytes;  // code byte -> two fp16 levels of V, kCopies times
+  static constexpr int kOffRef = kOffTab + 1024 * kCopies;                 // words of the rows, of two pieces in turn: negated references
+  static constexpr int kOffPos = kOffRef + 16 * NR;               //   (of both groups), position,
+  static constexpr int kOffSlope = kOffPos + 8 * NR;              //   slope x log2 e,
+  static constexpr int kOffMask = kOffSlope + 8 * NR;             //   64-bit ancestor mask
+  static constexpr int kOffFac = kOffMask + 16 * NR;              // 2 x NR floats: factors of a slow path
+  static constexpr int kOffMax = kOffFac + 8 * NR;                // 4 warps x (kStreams x NR) floats: maxima, sums
+  static constexpr int kOffCmb = kOffMax + 16 * NR * kStreams;               // 4 x NR floats: how the groups' results are put together
+  static constexpr int kOffVal = kOffCmb + 16 * NR;               // 8 tiles x 128 floats: log2 of the value norms
+  static constexpr int kOffLevels = kOffVal + 4096;               // 2 x 16 floats
   static constexpr int kOffBar = kOffLevels + 128;                // barriers, TMEM address, wait state, plan
   static constexpr int kSmemBytes = kOffBar + 320 + 1024;
   static_assert(kSmemBytes <= 232448, "one CTA's shared memory");
+  static_assert(8 * (kThreads / 32) <= 1024 * kCopies, "the prologue's scan words fit the table's");
 };
-constexpr int kKFull = 0, kVFull = 2, kSFull = 4, kSEmpty = 6, kPFull = 8, kPvDone = 10, kQFull = 12, kDrained = 13, kRingFull = 14, kRingEmpty = 20;
-constexpr int kOffTmemAddr = 208, kOffWait = 216, kOffPlan = 232, kOffValid = 256;   // inside kOffBar; valid: keys of each ring stage
+constexpr int kKFull = 0, kKEmpty = 2, kVFull = 4, kSFull = 6, kSEmpty = 10, kPFull = 14, kPvDone = 16, kQFull = 18, kDrained = 19, kRingFull = 20, kRingEmpty = 24;
+constexpr int kOffTmemAddr = 224, kOffWait = 232, kOffPlan = 248, kOffPlanEnd = 264, kOffValid = 272;   // inside kOffBar; valid: keys of each ring stage
 
 // ---- shared memory access -----------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -75,6 +88,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {          // (not volatile: look-ups in a table that is complete)
+  uint32_t v;
+  asm("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
 __device__ __forceinline__ float lds_f(uint32_t a) {
@@ -92,6 +110,8 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 __device__ __forceinline__ uint32_t sw128(uint32_t row, uint32_t chunk) {   // byte offset inside a block of 128-byte rows
   return (row >> 3) * 1024u + (row & 7u) * 128u + ((chunk ^ (row & 7u)) << 4);
 }
+// Named barriers: 1 .. 4 the softmax groups, 5 all of them; 6 the V producers; 7, 8 the K producers.
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void group_barrier(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
 __device__ __forceinline__ bool group_any(int group, bool mine) {
   uint32_t r;
@@ -112,7 +132,8 @@ __device__ __forceinline__ float warp_max(float x) {
 }
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
-  if constexpr (N == 8) tmem_ld8(addr, v);
+  if constexpr (N == 4) tmem_ld4(addr, v);
+  else if constexpr (N == 8) tmem_ld8(addr, v);
   else tmem_ld16(addr, v);
 }
 template <int N>
@@ -121,29 +142,60 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[N]
   else tmem_st16(addr, v);
 }
 
-// A bounded wait for a barrier phase.  An attempt lets the hardware park the warp for up to kParkNs, so that waiting warps
-// leave the issue slots to the working ones (attempts without the hint, with the timer read between them, cost the
-// working warps three quarters of their speed).  Once a wait of the CTA has given up, every later one returns after one
-// attempt: all roles then run their loops to the end (so nobody is left at a named barrier) without issuing or writing.
-constexpr uint32_t kParkNs = 20000;
-__device__ __forceinline__ bool park_wait(uint32_t bar, uint32_t parity) {
+// A bounded wait for a barrier phase.  Attempts carry no time hint (with one, an attempt is a software loop that sleeps: it
+// wakes late and takes issue slots), and abort flag and clock are read after every eight.  Once a wait of the CTA has given up,
+// every later one does so after eight attempts: all roles then run their loops to the end (so nobody is left at a named
+// barrier) without issuing or writing anything.
+__device__ __forceinline__ bool try_eight(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra D;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "D:\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(kParkNs)
+      : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0;
 }
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile WaitState* ws) {
-  if (park_wait(bar, parity)) return true;
+  if (try_eight(bar, parity)) return true;
   const unsigned long long t0 = global_timer_ns();
-  while (!ws->abort && global_timer_ns() - t0 < ws->limit_ns)
-    if (park_wait(bar, parity)) return true;
+#pragma unroll 1
+  while (!ws->abort && global_timer_ns() - t0 <= ws->limit_ns)
+    if (try_eight(bar, parity)) return true;
   ws->abort = 1;
   return false;
+}
+
+// Sums of M values per lane over the warp's 32 lanes: lane l returns the total of value l % M (M - 1 + log2(32 / M) exchanges
+// where one butterfly per value would take 5 M).
+template <int M>
+__device__ __forceinline__ float transposed_sum(float (&v)[M], int lane) {
+#pragma unroll
+  for (int d = M / 2; d > 0; d >>= 1) {
+    const bool upper = (lane & d) != 0;
+#pragma unroll
+    for (int j = 0; j < d; ++j) v[j] = (upper ? v[j + d] : v[j]) + __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j + d], d);
+  }
+#pragma unroll
+  for (int d = M; d < 32; d <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+  return v[0];
+}
+template <int R>
+__device__ __forceinline__ void raise_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void lower_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 // ---- the walk over segments ---------------------------------------------------------------------------------------------
@@ -207,48 +259,62 @@ struct Space {
   }
 };
 
-// Share of this CTA: finds its first segment and tile.  Every thread takes part.
+// Share of this CTA.  All segments are laid end to end, each with kPieceCost empty positions in front of its tiles, and the line
+// is cut into equal parts: CTAs that serve more segments get fewer tiles.  s_plan: first entry, head, tile; s_end: tiles.
 template <int NR, int THREADS>
-__device__ __forceinline__ void find_share(const AttendParams& p, int* s_scan, int* s_plan) {
+__device__ __forceinline__ void find_share(const AttendParams& p, int2* s_scan, int* s_plan, int* s_end) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, entries = p.B * p.row_blocks;
   const int per = (entries + THREADS - 1) / THREADS, e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
-  int sum = 0;
+  int tiles = 0, used = 0;                                       // of this thread's entries, one head: tiles, entries with any
   for (int e = e0; e < e1; ++e) {
-    sum += entry_of<NR>(p, e).tiles * p.H_kv;
+    const int n = entry_of<NR>(p, e).tiles;
+    tiles += n;
+    used += n > 0;
     if (blockIdx.x == 0 && e % p.row_blocks == 0 && sequence_view(p, e / p.row_blocks).bad) atomicOr(&g_tree_status, kStatusLengths);
   }
-  int x = sum;
+  int x = tiles, y = used;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, d);
-    if (lane >= d) x += y;
+    const int u = __shfl_up_sync(0xffffffffu, x, d), v = __shfl_up_sync(0xffffffffu, y, d);
+    if (lane >= d) { x += u; y += v; }
   }
-  if (lane == 31) s_scan[warp] = x;
-  if (tid == 0) s_plan[3] = 0;
+  if (lane == 31) s_scan[warp] = make_int2(x, y);
   __syncthreads();
-  int before = x - sum, total = 0;
+  int tiles_before = x - tiles, used_before = y - used, all_tiles = 0, all_used = 0;
   for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
+    const int2 s = s_scan[w];
+    if (w < warp) { tiles_before += s.x; used_before += s.y; }
+    all_tiles += s.x;
+    all_used += s.y;
   }
-  // the first `busy` CTAs take equal shares of at least one tile, so the pieces of a segment lie in consecutive CTAs
-  const int busy = min(static_cast<int>(gridDim.x), total), cta = min(static_cast<int>(blockIdx.x), busy);
-  const int lo = busy ? static_cast<int>(static_cast<int64_t>(total) * cta / busy) : 0;
-  const int hi = cta < busy ? static_cast<int>(static_cast<int64_t>(total) * (cta + 1) / busy) : lo;
-  if (hi > lo && before <= lo && lo < before + sum) {
-    int at = before;
+  const int64_t line = static_cast<int64_t>(all_tiles + kPieceCost * all_used) * p.H_kv;
+  const int busy = static_cast<int>(line < gridDim.x ? line : gridDim.x), cta = min(static_cast<int>(blockIdx.x), busy);
+  const int64_t lo = busy ? line * cta / busy : 0, hi = cta < busy ? line * (cta + 1) / busy : lo;
+  if (tid == 0) s_plan[3] = *s_end = 0;
+  __syncthreads();
+  int64_t at = static_cast<int64_t>(tiles_before + kPieceCost * used_before) * p.H_kv;
+  const int64_t mine = static_cast<int64_t>(tiles + kPieceCost * used) * p.H_kv;
+  if (hi > lo && hi > at && lo < at + mine) {                    // the line's positions lo or hi - 1 may lie in these entries
+    int real = tiles_before * p.H_kv;
     for (int e = e0; e < e1; ++e) {
-      const int tiles = entry_of<NR>(p, e).tiles;
-      if (lo < at + tiles * p.H_kv) {
-        s_plan[0] = e;
-        s_plan[1] = (lo - at) / tiles;
-        s_plan[2] = (lo - at) % tiles;
-        s_plan[3] = hi - lo;
-        break;
+      const int n = entry_of<NR>(p, e).tiles, len = n + kPieceCost;
+      if (n == 0) continue;
+      const int64_t next = at + static_cast<int64_t>(len) * p.H_kv;
+      if (at <= lo && lo < next) {
+        const int h = static_cast<int>(lo - at) / len, j = max(static_cast<int>(lo - at) % len - kPieceCost, 0);
+        s_plan[0] = e; s_plan[1] = h; s_plan[2] = j;
+        s_plan[3] = real + h * n + j;
       }
-      at += tiles * p.H_kv;
+      if (at < hi && hi <= next) {
+        const int h = static_cast<int>(hi - at) / len, j = max(static_cast<int>(hi - at) % len - kPieceCost, 0);
+        *s_end = real + h * n + j;
+      }
+      at = next;
+      real += n * p.H_kv;
     }
   }
+  __syncthreads();
+  if (tid == 0) s_plan[3] = *s_end - s_plan[3];
   __syncthreads();
 }
 
@@ -278,19 +344,20 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
   const uint32_t bar0 = base + C::kOffBar;
   auto bar = [&](int i) { return bar0 + 8u * i; };
 
-  find_share<NR, C::kThreads>(p, reinterpret_cast<int*>(sm + C::kOffMax), s_plan);
+  find_share<NR, C::kThreads>(p, reinterpret_cast<int2*>(sm + C::kOffTab), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kOffPlanEnd));
   const int total = s_plan[3];
   if (total == 0) {
     if (tid == 0) space.rec[blockIdx.x] = Record{-1, 0, 0, 0};
     return;
   }
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kKFull + i), 4); mbar_init(bar(kVFull + i), 4); mbar_init(bar(kSFull + i), 1);
-      mbar_init(bar(kSEmpty + i), C::kSoftWarps); mbar_init(bar(kPFull + i), C::kSoftWarps); mbar_init(bar(kPvDone + i), 1);
+    for (int i = 0; i < 2; ++i) {                               // counts: warps that arrive, or one commit
+      mbar_init(bar(kKFull + i), 4); mbar_init(bar(kKEmpty + i), 1); mbar_init(bar(kVFull + i), 4);
+      mbar_init(bar(kPFull + i), C::kSoftWarps / C::kStreams); mbar_init(bar(kPvDone + i), 1);
     }
+    for (int i = 0; i < C::kSBuffers; ++i) { mbar_init(bar(kSFull + i), 1); mbar_init(bar(kSEmpty + i), C::kSoftWarps / C::kStreams); }
     mbar_init(bar(kQFull), C::kSoftWarps);
-    mbar_init(bar(kDrained), 1);
+    mbar_init(bar(kDrained), 2);
     for (int i = 0; i < C::kRing; ++i) { mbar_init(bar(kRingFull + i), 1); mbar_init(bar(kRingEmpty + i), 8); }
     wait->abort = 0;
     wait->limit_ns = kWaitLimitNs;
@@ -300,7 +367,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     const int side = tid >> 4, i = tid & 15, n = (side ? p.v_bits : p.k_bits) == 4 ? 16 : 4;
     reinterpret_cast<float*>(sm + C::kOffLevels)[tid] = i < n ? __ldg((side ? p.cb_v : p.cb_k) + i) : 0.f;
   }
-  if (warp == C::kWarpMma) {
+  if (warp == C::kWarpS) {
     tmem_alloc(base + C::kOffBar + kOffTmemAddr, C::kTmemCols);
     tmem_relinquish();
   }
@@ -312,311 +379,438 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
   Record rec{-1, 0, 0, 0};
 
   if (warp < C::kSoftWarps) {
-    // ============ softmax: a thread is a key (TMEM lane), its group's rows are columns ======================================
-    const int group = warp >> 2, key = (warp & 3) * 32 + lane, gtid = tid & 127, col0 = group * C::kCols;
+    // ============ softmax: a thread is a key (tensor-memory lane), the rows of the block are columns.  Two groups share a tile,
+    // half of the columns each, and the pairs take tiles in turn, each with its own references, sums and O: a group's chain of
+    // waits and barriers spans two tiles =====================================================================================
+    raise_registers<C::kRegsSoft>();
+    const int group = warp >> 2, stream = C::kStreams == 2 ? group & 1 : 0, col0 = (C::kStreams == 2 ? group >> 1 : group) * C::kCols;
+    const int own0 = col0 + stream * C::kOwn;
+    const int key = (warp & 3) * 32 + lane, gtid = tid & 127;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t ref_a = base + C::kOffRef + 4 * col0, fac_a = base + C::kOffFac + 4 * col0, max_a = base + C::kOffMax + 16 * col0;
+    const uint32_t fac_a = base + C::kOffFac + 4 * C::kCols * group, max_a = base + C::kOffMax + 16 * C::kCols * group;
     const float kf = p.scale * kLog2e, cap2 = p.softcap * kLog2e, inv_cap = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
-    bool alive = true;
-    int i = 0;                                                  // tiles so far, over all pieces
-    Piece pc;
-    while (w.next(p, pc)) {
-      const Entry& x = pc.x;
-      // ---- the group's query rows: rotate, split, store as the B operand; what the masks need of them
-#pragma unroll 1
-      for (int r0 = warp & 3; r0 < C::kCols; r0 += 16) {        // four rows at a time
-        float q[4][4];
-        int t[4];
+    constexpr int kRowsWarp = C::kOwn / 4;
+    auto place = [&](const Piece& q, int r, int& t) {           // row r of the block: its token, and its index in (T, H_q)
+      const int row = q.x.rb * NR + r;
+      t = p.group == 1 ? row : static_cast<int>(__umulhi(static_cast<uint32_t>(row), p.group_magic));
+      return static_cast<int64_t>(q.x.q_begin + t) * p.H_q + q.head * p.group + (row - t * p.group);
+    };
+    // The query rows and row words of a piece are prepared by the group that owns the rows: loads first, the rest later.
+    auto load_rows = [&](const Piece& q, uint2 (&rows)[kRowsWarp]) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = col0 + r0 + 4 * u, row = x.rb * NR + r;
-          t[u] = row / p.group;
-          q[u][0] = q[u][1] = q[u][2] = q[u][3] = 0.f;
-          if (r0 + 4 * u < C::kCols && t[u] < x.q_len)
-            load_half4(p.q + (static_cast<int64_t>(x.q_begin + t[u]) * p.H_q + pc.head * p.group + row % p.group) * kHeadDim + 4 * lane, q[u]);
+      for (int u = 0; u < kRowsWarp; ++u) {
+        int t;
+        const int64_t at = place(q, own0 + 4 * u + (warp & 3), t);
+        rows[u] = make_uint2(0u, 0u);
+        if (t < q.x.q_len) rows[u] = __ldg(reinterpret_cast<const uint2*>(p.q + at * kHeadDim) + lane);
+      }
+    };
+    auto prepare_rows = [&](const Piece& q, const uint2 (&rows)[kRowsWarp], int set) {
+      if (gtid < C::kOwn) {
+        int t;
+        const int64_t at = place(q, own0 + gtid, t);
+        const bool real = t < q.x.q_len;
+        const int r = set * NR + own0 + gtid;
+        const unsigned long long m = real && p.tree_mask ? static_cast<unsigned long long>(p.tree_mask[q.x.q_begin + t]) : 0ull;
+        reinterpret_cast<unsigned long long*>(sm + C::kOffMask)[r] = m;
+        reinterpret_cast<int*>(sm + C::kOffPos)[r] = q.x.ctx + (!real ? 0 : p.tree_mask ? max(__popcll(m) - 1, 0) : t);
+        reinterpret_cast<float*>(sm + C::kOffSlope)[r] = p.slopes && real ? p.slopes[at % p.H_q] * kLog2e : 0.f;
+        float* ref = reinterpret_cast<float*>(sm + C::kOffRef) + 2 * set * NR + own0 + gtid;
+        ref[0] = ref[NR] = kNoRef;
+      }
+      constexpr int kBatch = kRowsWarp < 4 ? kRowsWarp : 4;
+#pragma unroll
+      for (int u0 = 0; u0 < kRowsWarp; u0 += kBatch) {
+        float f[kBatch][4];
+#pragma unroll
+        for (int v = 0; v < kBatch; ++v) {
+          const __half2 a = *reinterpret_cast<const __half2*>(&rows[u0 + v].x), b = *reinterpret_cast<const __half2*>(&rows[u0 + v].y);
+          f[v][0] = __low2float(a); f[v][1] = __high2float(a); f[v][2] = __low2float(b); f[v][3] = __high2float(b);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = col0 + r0 + 4 * u;
-          if (r0 + 4 * u >= C::kCols) break;
-          fht128_warp(q[u], lane);
+        for (int v = 0; v < kBatch; ++v) fht128_warp(f[v], lane);
+#pragma unroll
+        for (int v = 0; v < kBatch; ++v) {
           float lo[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            q[u][c] *= kRsqrtD;
-            lo[c] = q[u][c] - round_to_half(q[u][c]);
+            f[v][c] *= kRsqrtD;
+            lo[c] = f[v][c] - round_to_half(f[v][c]);
           }
-          const uint2 h = pack_half4(q[u]), l = pack_half4(lo);
-          const uint32_t at = base + C::kOffQ + (lane >> 4) * (NR * 128) + sw128(r, (lane & 15) >> 1) + 8 * (lane & 1);
+          const uint2 h = pack_half4(f[v]), l = pack_half4(lo);
+          const uint32_t at = base + C::kOffQ + (lane >> 4) * (NR * 128) + sw128(own0 + 4 * (u0 + v) + (warp & 3), (lane & 15) >> 1) + 8 * (lane & 1);
           sts64(at, h.x, h.y);
           sts64(at + NR * 256, l.x, l.y);
-          if (lane == 0) {
-            const bool real = t[u] < x.q_len;
-            reinterpret_cast<int*>(sm + C::kOffPos)[r] = x.ctx + (real ? depth_of(p, x.q_begin, t[u]) : 0);
-            reinterpret_cast<unsigned long long*>(sm + C::kOffMask)[r] =
-                real && p.tree_mask ? static_cast<unsigned long long>(p.tree_mask[x.q_begin + t[u]]) : 0ull;
-            reinterpret_cast<float*>(sm + C::kOffSlope)[r] =
-                p.slopes ? p.slopes[pc.head * p.group + (x.rb * NR + r) % p.group] * kLog2e : 0.f;
-            sts_f(ref_a + 4 * (r - col0), kNoRef);
-          }
         }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kQFull));
-      group_barrier(group);                                     // the rows' words are read by the whole group
+    };
+    const int my_o = C::kColO + stream * NR + col0;
+    int done = 0, set = 0;                                      // tiles of the pieces so far; which set of row words
+    Piece pc, nx;
+    uint2 rows[kRowsWarp];
+    bool more = w.next(p, pc);
+    if (more) {
+      load_rows(pc, rows);
+      prepare_rows(pc, rows, set);
+    }
+    while (more) {
+      named_barrier(5, 512);                                    // the row words of both groups
+      const int ctx = pc.x.ctx, seq_len = pc.x.seq_len, end = done + pc.n;
+      const uint32_t ref_a = base + C::kOffRef + 4 * ((2 * set + stream) * NR + col0);
+      const int* pos_w = reinterpret_cast<const int*>(sm + C::kOffPos) + set * NR + col0;
+      const float* slope_w = reinterpret_cast<const float*>(sm + C::kOffSlope) + set * NR + col0;
+      const uint32_t* mask_w = reinterpret_cast<const uint32_t*>(sm + C::kOffMask) + 2 * (set * NR + col0);
+      // tiles (by their number in all pieces) whose keys every row sees: [see_lo, see_hi)
+      const int tile_at = pc.tile0 - done;                      // key tile = number + tile_at
+      const int see_hi = p.slopes ? done : (ctx + (p.tree_mask ? 0 : pc.x.t0 + 1)) / kKeys - tile_at;
+      const int see_lo = p.window > 0 ? max(0, ctx + pc.x.q_len - p.window + kKeys) / kKeys - tile_at : done;
       uint64_t sum[C::kCols / 2];
 #pragma unroll
       for (int c = 0; c < C::kCols / 2; ++c) sum[c] = f2_pack(0.f, 0.f);
+      uint32_t s[C::kBlock];                                    // raw scores of the next tile's first block, in flight
+      auto fetch = [&](int tile) {
+        if ((warp & 3) == 0) wait_for(bar(kSFull + (tile & (C::kSBuffers - 1))), (tile >> C::kSShift) & 1, wait);
+        if (C::kStreams == 2 && (warp & 3) == 1 && tile >= 2) wait_for(bar(kPvDone + stream), ((tile - 2) >> 1) & 1, wait);   // P and O of the stream's last tile are at rest
+        group_barrier(group);
+        tc_fence_after_sync();
+        tmem_load<C::kBlock>(lanes + C::kColS + (tile & (C::kSBuffers - 1)) * NR + col0, s);
+      };
+      int i = C::kStreams == 2 ? done + ((done ^ stream) & 1) : done;     // this group's tiles: those of its parity, or all
+      const bool any_tile = i < end;
+      if (any_tile) fetch(i);
 
 #pragma unroll 1
-      for (int k = 0; k < pc.n; ++k, ++i) {
-        const int key0 = (pc.tile0 + k) * kKeys;
-        alive = wait_for(bar(kSFull + (i & 1)), (i >> 1) & 1, wait) && alive;
-        __syncwarp();
-        tc_fence_after_sync();
-        const uint32_t s_col = lanes + C::kColS + (i & 1) * NR + col0;
-        // some row may not see some key of this tile, or keys get a bias: the scores are finished here, one by one
-        const bool rule = p.slopes != nullptr || key0 + kKeys > x.ctx + (p.tree_mask ? 0 : x.t0 + 1) ||
-                          (p.window > 0 && key0 <= x.ctx + x.q_len - p.window);
-        const bool finish = rule || p.softcap > 0.f;
-        const float f = finish ? 1.0f : kf;
-        const uint64_t ff = f2_pack(f, f);
-        const int n = key0 + key;
-        int pos_k = n;
-        if (rule && p.tree_mask && n >= x.ctx && n < x.seq_len) pos_k = x.ctx + depth_of(p, x.q_begin, n - x.ctx);
-        // pass 1: does any score exceed its row's reference by more than an fp16 probability can carry?
-        float excess = -INFINITY;
-#pragma unroll
-        for (int ch = 0; ch < C::kChunks; ++ch) {
-          uint32_t s[C::kChunk];
-          tmem_load<C::kChunk>(s_col + ch * C::kChunk, s);
-          tmem_wait_ld();
-          if (finish) {
-#pragma unroll
-            for (int c = 0; c < C::kChunk; ++c) {
-              const int r = col0 + ch * C::kChunk + c;
-              float v = __uint_as_float(s[c]);
-              v = p.softcap > 0.f ? cap2 * soft_tanh(v * inv_cap) : v * kf;
-              if (rule) {
-                const int pos_q = reinterpret_cast<const int*>(sm + C::kOffPos)[r];
-                v = fmaf(reinterpret_cast<const float*>(sm + C::kOffSlope)[r], static_cast<float>(pos_k - pos_q), v);
-                bool see = n < x.ctx;
-                if (!see && n < x.seq_len)
-                  see = p.tree_mask ? (reinterpret_cast<const unsigned long long*>(sm + C::kOffMask)[r] >> (n - x.ctx)) & 1ull : n <= pos_q;
-                if (p.window > 0 && pos_q - pos_k >= p.window) see = false;
-                v = see ? v : -INFINITY;
-              }
-              s[c] = __float_as_uint(v);
-            }
-            tmem_store<C::kChunk>(s_col + ch * C::kChunk, s);
-          }
-#pragma unroll
-          for (int c = 0; c < C::kChunk; c += 4) {
-            const uint4 r = lds128(ref_a + 4 * (ch * C::kChunk + c));
-            float a0, a1, a2, a3;
-            f2_unpack(f2_fma(f2_pack(s[c], s[c + 1]), ff, f2_pack(r.x, r.y)), a0, a1);
-            f2_unpack(f2_fma(f2_pack(s[c + 2], s[c + 3]), ff, f2_pack(r.z, r.w)), a2, a3);
-            excess = fmax3(excess, a0, a1);
-            excess = fmax3(excess, a2, a3);
-          }
-        }
-        if (finish) tmem_wait_st();
-        if (group_any(group, excess > kSafe)) {
-          // slow path: row maxima of the tile, new references, factors for what the rows hold already
+      for (bool first = true; i < end; i += C::kStreams, first = false) {
+        const bool rule = i >= see_hi || i < see_lo, finish = rule || p.softcap > 0.f;
+        if (finish) {                                           // cap, bias and masks, in the base-2 domain, eight columns at a time
+          const int n = (i + tile_at) * kKeys + key, j = n - ctx;
+          const int pos_k = rule && p.tree_mask && j >= 0 && n < seq_len ? ctx + depth_of(p, pc.x.q_begin, j) : n;
+          const int word = (j >> 5) & 1, up = 31 - (j & 31);    // bit j of a row's mask to the sign
+          const uint32_t all = j < 0 ? 0x80000000u : 0u, none = n < seq_len ? 0xffffffffu : 0u;
+          const float f1 = p.softcap > 0.f ? inv_cap : kf;
 #pragma unroll 1
-          for (int ch = 0; ch < C::kChunks; ++ch) {
-            uint32_t s[C::kChunk];
-            tmem_load<C::kChunk>(s_col + ch * C::kChunk, s);
+          for (int c0 = 0; c0 < C::kCols; c0 += 8) {
+            const uint32_t at = lanes + C::kColS + (i & (C::kSBuffers - 1)) * NR + col0 + c0;
+            uint32_t x[8];
+            tmem_load<8>(at, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < C::kChunk; ++c) {
-              const float m = warp_max(__uint_as_float(s[c]) * f);
-              if (lane == 0) sts_f(max_a + 4 * ((warp & 3) * C::kCols + ch * C::kChunk + c), m);
-            }
-          }
-          group_barrier(group);
-          if (gtid < C::kCols) {
-            float m = lds_f(max_a + 4 * gtid);
+            for (int c = 0; c < 8; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * f1);
+            if (p.softcap > 0.f) {
 #pragma unroll
-            for (int u = 1; u < 4; ++u) m = fmaxf(m, lds_f(max_a + 4 * (u * C::kCols + gtid)));
-            const float old = lds_f(ref_a + 4 * gtid);
-            float fac = 1.0f;
-            if (m + old > kSafe) {
-              fac = old == kNoRef ? 0.f : fast_exp2(-old - m);
-              sts_f(ref_a + 4 * gtid, -m);
+              for (int c = 0; c < 8; ++c) x[c] = __float_as_uint(cap2 * soft_tanh(__uint_as_float(x[c])));
             }
-            sts_f(fac_a + 4 * gtid, fac);
-          }
-          group_barrier(group);
+            if (rule) {
+              if (p.slopes) {
 #pragma unroll
-          for (int c = 0; c < C::kCols; c += 4) {
-            const uint4 r = lds128(fac_a + 4 * c);
-            sum[c / 2] = f2_mul(sum[c / 2], f2_pack(r.x, r.y));
-            sum[c / 2 + 1] = f2_mul(sum[c / 2 + 1], f2_pack(r.z, r.w));
+                for (int c = 0; c < 8; ++c) x[c] = __float_as_uint(fmaf(slope_w[c0 + c], static_cast<float>(pos_k - pos_w[c0 + c]), __uint_as_float(x[c])));
+              }
+              if (p.window > 0) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) x[c] = pos_w[c0 + c] - pos_k >= p.window ? 0xff800000u : x[c];
+              }
+              if (p.tree_mask) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) x[c] = static_cast<int>(((mask_w[2 * (c0 + c) + word] << up) | all) & none) < 0 ? x[c] : 0xff800000u;
+              } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) x[c] = n > pos_w[c0 + c] || n >= seq_len ? 0xff800000u : x[c];
+              }
+            }
+            tmem_store<8>(at, x);
           }
-          if (k > 0) {                                          // O of the piece so far; P V of this tile waits for this group
-            alive = wait_for(bar(kPvDone + ((i - 1) & 1)), ((i - 1) >> 1) & 1, wait) && alive;
-            __syncwarp();
-            tc_fence_after_sync();
-            const uint32_t o_col = lanes + C::kColO + col0;
+          tmem_wait_st();
+          tmem_load<C::kBlock>(lanes + C::kColS + (i & (C::kSBuffers - 1)) * NR + col0, s);      // instead of the raw ones
+        }
+        const uint64_t ff = f2_pack(finish ? 1.0f : kf, finish ? 1.0f : kf);
+        // the norm of a 4-bit value row rides on the probability: P = exp2(x + log2 norm - reference), p = P / norm
+        const float lg = lds_f(base + C::kOffVal + 4 * ((i & 7) * kKeys + key));
+        const uint32_t p_tile = base + C::kOffP + (C::kStreams == 2 ? stream : col0 >> 6) * kColBlock;
+#pragma unroll
+        for (int blk = 0; blk < C::kCols / C::kBlock; ++blk) {
+          const int c0 = blk * C::kBlock;
+          float e[C::kBlock];
 #pragma unroll 1
-            for (int ch = 0; ch < C::kChunks; ++ch) {
-              uint32_t o[C::kChunk];
-              tmem_load<C::kChunk>(o_col + ch * C::kChunk, o);
-              tmem_wait_ld();
+          for (bool again = false;; again = true) {
+            if (blk > 0 || again) tmem_load<C::kBlock>(lanes + C::kColS + (i & (C::kSBuffers - 1)) * NR + col0 + c0, s);
+            tmem_wait_ld();
+            if (again) {
+              // slow path: row maxima of the tile, new references, factors for what the rows hold already
 #pragma unroll
-              for (int c = 0; c < C::kChunk; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * lds_f(fac_a + 4 * (ch * C::kChunk + c)));
-              tmem_store<C::kChunk>(o_col + ch * C::kChunk, o);
+              for (int c = 0; c < C::kBlock; ++c) {
+                const float m = warp_max(fmaf(__uint_as_float(s[c]), finish ? 1.0f : kf, lg));
+                if (lane == 0) sts_f(max_a + 4 * ((warp & 3) * C::kCols + c), m);
+              }
+              group_barrier(group);
+              if (gtid < C::kBlock) {
+                float m = lds_f(max_a + 4 * gtid);
+#pragma unroll
+                for (int u = 1; u < 4; ++u) m = fmaxf(m, lds_f(max_a + 4 * (u * C::kCols + gtid)));
+                const float old = lds_f(ref_a + 4 * (c0 + gtid));
+                float fac = 1.0f;
+                if (m + old > kSafe) {
+                  fac = old == kNoRef ? 0.f : fast_exp2(-old - m);
+                  sts_f(ref_a + 4 * (c0 + gtid), -m);
+                }
+                sts_f(fac_a + 4 * (c0 + gtid), fac);
+              }
+              group_barrier(group);
             }
-            tmem_wait_st();
+            // probabilities against the references as they are; `excess`: the largest exponent
+            float excess = -INFINITY;
+            const uint64_t lg2 = f2_pack(lg, lg);
+#pragma unroll
+            for (int c = 0; c < C::kBlock; c += 4) {
+              const uint4 r = lds128(ref_a + 4 * (c0 + c));
+              float* a = e + c;
+              f2_unpack(f2_fma(f2_pack(s[c], s[c + 1]), ff, f2_add(f2_pack(r.x, r.y), lg2)), a[0], a[1]);
+              f2_unpack(f2_fma(f2_pack(s[c + 2], s[c + 3]), ff, f2_add(f2_pack(r.z, r.w), lg2)), a[2], a[3]);
+              excess = fmax3(excess, a[0], a[1]);
+              excess = fmax3(excess, a[2], a[3]);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) a[u] = fast_exp2(a[u]);
+            }
+            if (C::kStreams == 1 && blk == 0 && !again && i >= 1) {       // P and O of the last tile are at rest
+              if ((warp & 3) == 0) wait_for(bar(kPvDone + ((i - 1) & 1)), ((i - 1) >> 1) & 1, wait);
+              group_barrier(group);
+              tc_fence_after_sync();
+            }
+#pragma unroll
+            for (int c = 0; c < C::kBlock; c += 8)
+              sts128(p_tile + sw128(key, ((col0 & 63) + c0 + c) / 8), pack_half2(e[c], e[c + 1]), pack_half2(e[c + 2], e[c + 3]),
+                     pack_half2(e[c + 4], e[c + 5]), pack_half2(e[c + 6], e[c + 7]));
+            if (again) {
+#pragma unroll
+              for (int c = 0; c < C::kBlock; c += 4) {
+                const uint4 r = lds128(fac_a + 4 * (c0 + c));
+                sum[(c0 + c) / 2] = f2_mul(sum[(c0 + c) / 2], f2_pack(r.x, r.y));
+                sum[(c0 + c) / 2 + 1] = f2_mul(sum[(c0 + c) / 2 + 1], f2_pack(r.z, r.w));
+              }
+              if (!first) {                                     // O of the group's tiles so far (at rest, see fetch)
+                uint32_t o[C::kBlock];
+                tmem_load<C::kBlock>(lanes + my_o + c0, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < C::kBlock; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * lds_f(fac_a + 4 * (c0 + c)));
+                tmem_store<C::kBlock>(lanes + my_o + c0, o);
+                tmem_wait_st();
+              }
+              break;
+            }
+            if (!group_any(group, excess > kSafe)) break;
           }
-        }
-        // pass 2: probabilities against the references, sums in fp32, P to shared memory once its buffer is free
-        if (i >= C::kPStages) {
-          const int j = i - C::kPStages;
-          alive = wait_for(bar(kPvDone + (j & 1)), (j >> 1) & 1, wait) && alive;
-          __syncwarp();
-        }
-        const uint32_t p_tile = base + C::kOffP + (C::kPStages == 2 ? (i & 1) * C::kPBytes : 0) + (col0 >> 6) * kColBlock;
+          const float inv = fast_exp2(-lg);
+          const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
-        for (int ch = 0; ch < C::kChunks; ++ch) {
-          uint32_t s[C::kChunk], pk[C::kChunk / 2];
-          tmem_load<C::kChunk>(s_col + ch * C::kChunk, s);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < C::kChunk; c += 4) {
-            const uint4 r = lds128(ref_a + 4 * (ch * C::kChunk + c));
-            float a[4];
-            f2_unpack(f2_fma(f2_pack(s[c], s[c + 1]), ff, f2_pack(r.x, r.y)), a[0], a[1]);
-            f2_unpack(f2_fma(f2_pack(s[c + 2], s[c + 3]), ff, f2_pack(r.z, r.w)), a[2], a[3]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) a[u] = fast_exp2(a[u]);
-            const int g = (ch * C::kChunk + c) / 2;
-            sum[g] = f2_add(sum[g], f2_pack(a[0], a[1]));
-            sum[g + 1] = f2_add(sum[g + 1], f2_pack(a[2], a[3]));
-            pk[c / 2] = pack_half2(a[0], a[1]);
-            pk[c / 2 + 1] = pack_half2(a[2], a[3]);
-          }
-#pragma unroll
-          for (int c8 = 0; c8 < C::kChunk / 8; ++c8)
-            sts128(p_tile + sw128(key, ((col0 & 63) + ch * C::kChunk) / 8 + c8), pk[4 * c8], pk[4 * c8 + 1], pk[4 * c8 + 2], pk[4 * c8 + 3]);
+          for (int c = 0; c < C::kBlock; c += 2) sum[(c0 + c) / 2] = f2_fma(f2_pack(e[c], e[c + 1]), inv2, sum[(c0 + c) / 2]);
         }
         fence_async_smem();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(bar(kSEmpty + (i & 1)));
+          mbar_arrive(bar(kSEmpty + (i & (C::kSBuffers - 1))));
           mbar_arrive(bar(kPFull + (i & 1)));
         }
+        if (i + C::kStreams < end) fetch(i + C::kStreams);
       }
 
-      // ---- end of the piece: sums over the 128 keys, then O
-      alive = wait_for(bar(kPvDone + ((i - 1) & 1)), ((i - 1) >> 1) & 1, wait) && alive;
-      __syncwarp();
-      tc_fence_after_sync();
+      // ---- end of the piece.  The next piece's rows go first: its scores can then be computed while this one is written out
+      more = w.next(p, nx);
+      if (more) load_rows(nx, rows);
+      if (any_tile) {
 #pragma unroll
-      for (int c = 0; c < C::kCols; c += 2) {
-        float a, b;
-        f2_unpack(sum[c / 2], a, b);
-        a = warp_sum(a);
-        b = warp_sum(b);
-        if (lane == 0) {
-          sts_f(max_a + 4 * ((warp & 3) * C::kCols + c), a);
-          sts_f(max_a + 4 * ((warp & 3) * C::kCols + c + 1), b);
+        for (int c0 = 0; c0 < C::kCols; c0 += C::kBlock) {
+          float v[C::kBlock];
+#pragma unroll
+          for (int c = 0; c < C::kBlock; c += 2) f2_unpack(sum[(c0 + c) / 2], v[c], v[c + 1]);
+          const float l = transposed_sum<C::kBlock>(v, lane);
+          if (lane < C::kBlock) sts_f(max_a + 4 * ((warp & 3) * C::kCols + c0 + lane), l);
         }
       }
-      group_barrier(group);
-      if (gtid < C::kCols) {
-        float l = 0.f;
+      if ((warp & 3) == 0) {                                    // both S of this piece are done before Q is overwritten
+        const int last = end - 1, before = end - 2;
+        if (more) wait_for(bar(kSFull + (last & (C::kSBuffers - 1))), (last >> C::kSShift) & 1, wait);
+        if (any_tile) {
+          const int mine = C::kStreams == 1 || ((last ^ stream) & 1) == 0 ? last : before;
+          wait_for(bar(kPvDone + (mine & 1)), (mine >> 1) & 1, wait);
+        }
+      }
+      named_barrier(5, 512);
+      tc_fence_after_sync();
+      if (more) prepare_rows(nx, rows, set ^ 1);
+      // the two streams of every own row: sums, common reference, factors
+      const bool both = C::kStreams == 2 && pc.n > 1, only = C::kStreams == 2 && (done & 1) != 0;       // with a single tile one stream is empty
+      float* cmb = reinterpret_cast<float*>(sm + C::kOffCmb);   // [factor 0, factor 1, sum, reference][NR]
+      if (gtid < C::kOwn) {
+        const int r = own0 + gtid;
+        const float* ref = reinterpret_cast<const float*>(sm + C::kOffRef) + 2 * set * NR + r;
+        float m[2], l[2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) l += lds_f(max_a + 4 * (u * C::kCols + gtid));
-        sts_f(fac_a + 4 * gtid, l);
+        for (int g = 0; g < 2; ++g) {
+          m[g] = -INFINITY;
+          l[g] = 0.f;
+          if (g < C::kStreams && (both || only == (g == 1))) {
+            const float* part = reinterpret_cast<const float*>(sm + C::kOffMax) + 4 * C::kCols * (C::kStreams == 2 ? (group & 2) + g : group) + (r - col0);
+            l[g] = part[0] + part[C::kCols] + part[2 * C::kCols] + part[3 * C::kCols];
+            m[g] = ref[g * NR] == kNoRef ? -INFINITY : -ref[g * NR];
+          }
+        }
+        const float top = fmaxf(m[0], m[1]);
+        const float f0 = m[0] == -INFINITY ? 0.f : exp2f(m[0] - top), f1 = m[1] == -INFINITY ? 0.f : exp2f(m[1] - top);
+        // (a row without a reference has the sum 0, or NaN from NaN scores, which the factor 0 keeps)
+        cmb[r] = f0;
+        cmb[NR + r] = f1;
+        cmb[2 * NR + r] = (m[0] == -INFINITY ? l[0] : f0 * l[0]) + (m[1] == -INFINITY ? l[1] : f1 * l[1]);
+        cmb[3 * NR + r] = top;
       }
       group_barrier(group);
-      const bool whole = pc.starts && pc.ends;
+      const bool alive = wait->abort == 0, whole = pc.starts && pc.ends;
       const int64_t slot = static_cast<int64_t>(2) * blockIdx.x + (pc.starts ? 1 : 0);
       if (!whole) {
         if (pc.starts) { rec.tail_e = pc.e; rec.tail_head = pc.head; }
         else rec.head_state = pc.ends ? 2 : 1;
-        if (gtid < C::kCols && alive) {
-          const float nref = lds_f(ref_a + 4 * gtid);
-          space.ml[slot * NR + col0 + gtid] = make_float2(nref == kNoRef ? -INFINITY : -nref, lds_f(fac_a + 4 * gtid));
-        }
+        if (gtid < C::kOwn && alive)
+          space.ml[slot * NR + own0 + gtid] = make_float2(cmb[3 * NR + own0 + gtid], cmb[2 * NR + own0 + gtid]);
       }
 #pragma unroll 1
-      for (int ch = 0; ch < C::kChunks; ++ch) {
-        uint32_t o[C::kChunk];
-        tmem_load<C::kChunk>(lanes + C::kColO + col0 + ch * C::kChunk, o);
-        tmem_wait_ld();
+      for (int ch = own0; ch < own0 + C::kOwn; ch += C::kChunk) {
+        float o[C::kChunk];
+        {
+          uint32_t a[C::kChunk];
+          tmem_load<C::kChunk>(lanes + C::kColO + (both || !only ? 0 : NR) + ch, a);
+          tmem_wait_ld();
+          const float* f = cmb + (both || !only ? 0 : NR) + ch;
+#pragma unroll
+          for (int c = 0; c < C::kChunk; ++c) o[c] = __uint_as_float(a[c]) * f[c];
+          if (both) {
+            tmem_load<C::kChunk>(lanes + C::kColO + NR + ch, a);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < C::kChunk; ++c) o[c] = fmaf(__uint_as_float(a[c]), cmb[NR + ch + c], o[c]);
+          }
+        }
         if (!whole) {                                           // un-normalised, one row of 128 per column
-          float* to = space.o + (slot * NR + col0 + ch * C::kChunk) * kHeadDim + key;
+          float* to = space.o + (slot * NR + ch) * kHeadDim + key;
           if (alive) {
 #pragma unroll
-            for (int c = 0; c < C::kChunk; ++c) to[c * kHeadDim] = __uint_as_float(o[c]);
+            for (int c = 0; c < C::kChunk; ++c) to[c * kHeadDim] = o[c];
           }
           continue;
         }
-        // transpose through the (idle) P buffer, rotate back in fp32, round once
+        // transpose through the (idle) P buffers, rotate back in fp32, round once
         const uint32_t area = base + C::kOffP + group * (C::kChunk * 512);
+        constexpr int kRowsChunk = C::kChunk / 4;
+        if (ch > own0) group_barrier(group);
 #pragma unroll
-        for (int c = 0; c < C::kChunk; ++c) sts_f(area + c * 512 + key * 4, __uint_as_float(o[c]));
+        for (int c = 0; c < C::kChunk; ++c) sts_f(area + c * 512 + key * 4, o[c]);
         group_barrier(group);
-#pragma unroll 1
-        for (int c = warp & 3; c < C::kChunk; c += 4) {
-          const int r = ch * C::kChunk + c, row = x.rb * NR + col0 + r, t = row / p.group;
-          const float l = lds_f(fac_a + 4 * r), inv = l > 0.f ? kRsqrtD / l : (l == 0.f ? 0.f : l);
-          const uint4 v4 = lds128(area + c * 512 + lane * 16);
-          float v[4] = {__uint_as_float(v4.x) * inv, __uint_as_float(v4.y) * inv, __uint_as_float(v4.z) * inv, __uint_as_float(v4.w) * inv};
-          fht128_warp(v, lane);
-          if (t < x.q_len && alive) {
-            const int64_t at = static_cast<int64_t>(x.q_begin + t) * p.H_q + pc.head * p.group + row % p.group;
-            *reinterpret_cast<uint2*>(p.out + at * kHeadDim + 4 * lane) = pack_half4(v);
+        float v[kRowsChunk][4];
+#pragma unroll
+        for (int u = 0; u < kRowsChunk; ++u) {
+          const float l = cmb[2 * NR + ch + 4 * u + (warp & 3)], inv = l > 0.f ? kRsqrtD / l : (l == 0.f ? 0.f : l);
+          const uint4 v4 = lds128(area + (4 * u + (warp & 3)) * 512 + lane * 16);
+          v[u][0] = __uint_as_float(v4.x) * inv; v[u][1] = __uint_as_float(v4.y) * inv;
+          v[u][2] = __uint_as_float(v4.z) * inv; v[u][3] = __uint_as_float(v4.w) * inv;
+        }
+#pragma unroll
+        for (int u = 0; u < kRowsChunk; ++u) fht128_warp(v[u], lane);
+#pragma unroll
+        for (int u = 0; u < kRowsChunk; ++u) {
+          const int r = ch + 4 * u + (warp & 3);
+          int t;
+          const int64_t at = place(pc, r, t);
+          if (t < pc.x.q_len && alive) {
+            *reinterpret_cast<uint2*>(p.out + at * kHeadDim + 4 * lane) = pack_half4(v[u]);
             if (p.lse_out && lane == 0) {
-              const float nref = lds_f(ref_a + 4 * r);
-              p.lse_out[at] = nref == kNoRef && l == 0.f ? -INFINITY : (log2f(l) - nref) * kLn2;
+              const float l = cmb[2 * NR + r];
+              p.lse_out[at] = l == 0.f ? -INFINITY : (log2f(l) + cmb[3 * NR + r]) * kLn2;
             }
           }
         }
-        group_barrier(group);
       }
-      group_barrier(group);                                     // the rows' words may be overwritten
+      tc_fence_before_sync();
+      named_barrier(5, 512);                                    // O and the P buffers may be overwritten
+      tc_fence_after_sync();
+      done = end;
+      pc = nx;
+      set ^= 1;
     }
-  } else if (warp < C::kWarpMma) {
-    // ============ producers: slot -> exact fp16 row; K to tensor memory (lane = key), V to shared memory (row = key) ==========
+  } else if (warp < C::kWarpS) {
+    // ============ producers: slot -> fp16 row; K to tensor memory (lane = key), V to shared memory (row = key).  Two groups of
+    // four warps for K, each with every second tile, and one for V; a thread expands one row.  The loops are kept short: unrolled
+    // over the row, they evict one another (and the softmax) from the instruction caches and everything runs 1.5 times slower ==
     const bool is_v = warp >= C::kWarpV;
+    if (is_v) lower_registers<C::kRegsV>();
+    else lower_registers<C::kRegsK>();
+    const int step = is_v ? 1 : 2, begin = is_v ? 0 : (warp >> 2) & 1;
     const int key = (warp & 3) * 32 + lane, bits = is_v ? p.v_bits : p.k_bits;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + C::kColK;
     const uint32_t cell0 = base + C::kOffRing + key * p.slot_bytes, code_at = is_v ? 16 * p.k_bits : 0;
-    const uint32_t norm_at = 16 * (p.k_bits + p.v_bits) + (is_v ? 4 : 0), row = base + C::kOffV;
+    const uint32_t norm_at = 16 * (p.k_bits + p.v_bits), row0 = base + C::kOffV;
     const float* levels = reinterpret_cast<const float*>(sm + C::kOffLevels) + (is_v ? 16 : 0);
-    const int full = is_v ? kVFull : kKFull, freed = is_v ? kPvDone : kSFull;
-    int stage = 0, turn = 0;
+    const uint32_t tab_a = base + C::kOffTab + 4 * (lane & (kCopies - 1));
+    if (is_v && bits == 4) {                                    // the V warps fill the value table
+      for (int k = tid - C::kWarpV * 32; k < 256 * kCopies; k += 128)
+        *reinterpret_cast<uint32_t*>(sm + C::kOffTab + 4 * k) = pack_half2(levels[k / (16 * kCopies)], levels[(k / kCopies) & 15]);
+    }
+    const int id = is_v ? 6 : 7 + begin;                        // named barriers: V 6; K 7, 8
+    int stage = begin, wraps = 0;                               // of the ring
 #pragma unroll 1
-    for (int i = 0; i < total; ++i) {
-      wait_for(bar(kRingFull + stage), turn, wait);
-      const uint32_t cell = cell0 + stage * kStageBytes;
-      const int valid = *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage);
-      const float norm = key < valid ? lds_f(cell + norm_at) : 0.f;       // keys past the end: zero rows
-      const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
-      if (i >= 2) wait_for(bar(freed + (i & 1)), ((i - 2) >> 1) & 1, wait);
-      __syncwarp();
+    for (int i = begin; i < total; i += step) {
+      const int buffer = i & 1, slot = (is_v ? kVFull : kKFull) + buffer;               // its "full" barrier
+      const uint32_t row = row0 + buffer * kTileBytes;
+      if ((warp & 3) == 0) {                                    // the slots are there, and the buffer they go to is free
+        wait_for(bar(kRingFull + stage), wraps & 1, wait);
+        if (i >= 2) wait_for(bar((is_v ? kPvDone : kKEmpty) + buffer), ((i - 2) >> 1) & 1, wait);
+      }
+      named_barrier(id, 128);
       tc_fence_after_sync();
+      const uint32_t cell = cell0 + stage * kStageBytes;
+      if (is_v && bits == 4) {
+        // 4-bit values: fp16 levels from the table, one look-up per code byte; the norm goes into the key's probabilities
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {                                        // 32 coordinates at a time
-        uint32_t v[16];
-        if (bits == 4) {
-          expand::quarter4(t, lds128(cell + code_at + 16 * c), v);
-        } else {
-          const uint2 w = lds64(cell + code_at + 8 * c);
-          expand::quarter2(t, w.x, w.y, v);
-        }
-        if (is_v) {
+        for (int c = 0; c < 4; ++c) {
+          const uint4 w4 = lds128(cell + code_at + 16 * c);
+          const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w}, to = row + (c >> 1) * kColBlock;
+          uint32_t v[16];                                       // all look-ups first: a store in between would wait for each
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            sts128(row + (i & 1) * kTileBytes + (c >> 1) * kColBlock + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-        } else {
-          tmem_st16(lanes + (i & 1) * 64 + 16 * c, v);
+          for (int u = 0; u < 4; ++u) {
+            v[4 * u] = lds32(tab_a + ((ws[u] << kRowShift) & kRowMask));
+            v[4 * u + 1] = lds32(tab_a + ((ws[u] >> (8 - kRowShift)) & kRowMask));
+            v[4 * u + 2] = lds32(tab_a + ((ws[u] >> (16 - kRowShift)) & kRowMask));
+            v[4 * u + 3] = lds32(tab_a + ((ws[u] >> (24 - kRowShift)) & kRowMask));
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sts128(to + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        }
+      } else {
+        const uint2 norms = lds64(cell + norm_at);
+        const bool live = key < *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage);
+        const float norm = live ? __uint_as_float(is_v ? norms.y : norms.x) : 0.f;        // keys past the end: zero rows
+        const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
+        if (!is_v) {                                                      // (eight tiles deep: read before S of tile i + 4 is written)
+          const float nv = fminf(fmaxf(__uint_as_float(norms.y), 1.0e-30f), 1.0e30f);
+          sts_f(base + C::kOffVal + 4 * ((i & 7) * kKeys + key), p.v_bits == 4 && live ? __log2f(nv) : 0.f);
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {                                     // 32 coordinates at a time
+          uint32_t v[16];
+          if (bits == 4) {
+            expand::quarter4(t, lds128(cell + code_at + 16 * c), v);
+          } else {
+            const uint2 w = lds64(cell + code_at + 8 * c);
+            expand::quarter2(t, w.x, w.y, v);
+          }
+          if (is_v) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              sts128(row + (c >> 1) * kColBlock + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+          } else {
+            tmem_st16(lanes + buffer * 64 + 16 * c, v);
+          }
         }
       }
       if (is_v) fence_async_smem();
@@ -625,97 +819,110 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(bar(kRingEmpty + stage));
-        mbar_arrive(bar(full + (i & 1)));
+        mbar_arrive(bar(slot));
       }
-      if (++stage == C::kRing) { stage = 0; turn ^= 1; }
+      stage += step;
+      if (stage >= C::kRing) { stage -= C::kRing; ++wraps; }
     }
-  } else if (warp == C::kWarpFeed) {
-    // ============ feeder: one lane per 16-token group of a tile; block ids are read one tile ahead ============================
-    Piece q;
-    bool live = w.next(p, q), bad = false, alive = true;
-    int tile = live ? q.tile0 : 0, stage = 0, turn = 0, issued = 0;
-    auto block_id = [&]() {
-      const int n = min(tile * kKeys + 16 * (lane & 7), q.x.seq_len - 1);
-      return __ldg(p.block_table + static_cast<int64_t>(q.x.b) * p.bt_stride + (p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size));
-    };
-    int id = live ? block_id() : 0;
+  } else {
+    lower_registers<C::kRegsOther>();
+    if (warp == C::kWarpFeed) {
+      // ============ feeder: one lane per 16-token group of a tile; block ids are read one tile ahead ============================
+      Piece q;
+      bool live = w.next(p, q), bad = false, alive = true;
+      int tile = live ? q.tile0 : 0, stage = 0, turn = 0, issued = 0;
+      auto block_id = [&]() {
+        const int n = min(tile * kKeys + 16 * (lane & 7), q.x.seq_len - 1);
+        return __ldg(p.block_table + static_cast<int64_t>(q.x.b) * p.bt_stride + (p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size));
+      };
+      int id = live ? block_id() : 0;
 #pragma unroll 1
-    while (live && alive) {
-      if (issued >= C::kRing) alive = wait_for(bar(kRingEmpty + stage), turn ^ 1, wait);
-      if (!__all_sync(0xffffffffu, alive)) break;
-      const int left = q.x.seq_len - tile * kKeys, groups = min(8, (left + 15) >> 4), n = tile * kKeys + 16 * lane;
-      if (lane == 0) {
-        *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage) = min(left, kKeys);
-        expect_bytes(bar(kRingFull + stage), groups * 16 * p.slot_bytes);
-      }
-      __syncwarp();
-      if (lane < groups) {
-        if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) { bad = true; id = 0; }
-        const int in = p.bs_shift >= 0 ? n & (p.block_size - 1) : n % p.block_size;
-        copy_group(base + C::kOffRing + stage * kStageBytes + lane * 16 * p.slot_bytes, &map, q.head * p.slot_bytes, id * p.block_size + in, bar(kRingFull + stage));
-      }
-      ++issued;
-      if (++stage == C::kRing) { stage = 0; turn ^= 1; }
-      if (++tile == q.tile0 + q.n) {
-        live = w.next(p, q);
-        if (live) tile = q.tile0;
-      }
-      if (live) id = block_id();
-    }
-    if (bad) atomicOr(&g_tree_status, kStatusBadBlock);
-    // no copy may be in flight when the CTA ends, also after a wait elsewhere gave up
-    const unsigned long long t0 = global_timer_ns();
-    for (int k = max(0, issued - C::kRing); k < issued; ++k)
-      while (!park_wait(bar(kRingFull + k % C::kRing), (k / C::kRing) & 1) && global_timer_ns() - t0 < kWaitLimitNs) { }
-  } else if (lane == 0) {
-    // ============ MMA issuer =================================================================================================
-    constexpr uint32_t idesc_s = instr_desc_f16(kKeys, NR, false, false), idesc_o = instr_desc_f16(kHeadDim, NR, true, true);
-    bool alive = true;
-    int i = 0, pieces = 0;
-    auto issue_s = [&](int x) {
-      alive = wait_for(bar(kKFull + (x & 1)), (x >> 1) & 1, wait) && alive;
-      if (x >= 2) alive = wait_for(bar(kSEmpty + (x & 1)), ((x - 2) >> 1) & 1, wait) && alive;
-      if (!alive) return;
-      tc_fence_after_sync();
-      const uint32_t d = tmem + C::kColS + (x & 1) * NR, a = tmem + C::kColK + (x & 1) * 64;
-#pragma unroll
-      for (int term = 0; term < 2; ++term)
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint64_t b = smem_desc_sw128(base + C::kOffQ + term * (NR * 256) + (ks >> 2) * (NR * 128) + (ks & 3) * 32u, 16, 1024);
-          if (term == 0 && ks == 0) mma_ts<false>(d, a, b, idesc_s);
-          else mma_ts<true>(d, a + 8 * ks, b, idesc_s);
+      while (live && alive) {
+        if (issued >= C::kRing) alive = wait_for(bar(kRingEmpty + stage), turn ^ 1, wait);
+        if (!__all_sync(0xffffffffu, alive)) break;
+        const int left = q.x.seq_len - tile * kKeys, groups = min(8, (left + 15) >> 4), n = tile * kKeys + 16 * lane;
+        if (lane == 0) {
+          *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage) = min(left, kKeys);
+          expect_bytes(bar(kRingFull + stage), groups * 16 * p.slot_bytes);
         }
-      mma_commit(bar(kSFull + (x & 1)));
-    };
-    auto issue_o = [&](int x, bool first) {
-      alive = wait_for(bar(kVFull + (x & 1)), (x >> 1) & 1, wait) && alive;
-      alive = wait_for(bar(kPFull + (x & 1)), (x >> 1) & 1, wait) && alive;
-      if (!alive) return;
-      tc_fence_after_sync();
-      const uint32_t v = base + C::kOffV + (x & 1) * kTileBytes, pt = base + C::kOffP + (C::kPStages == 2 ? (x & 1) * C::kPBytes : 0);
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks)
-        mma_ss(tmem + C::kColO, smem_desc_sw128(v + ks * 2048u, kColBlock, 1024), smem_desc_sw128(pt + ks * 2048u, kColBlock, 1024),
-               idesc_o, first && ks == 0 ? 0u : 1u);
-      mma_commit(bar(kPvDone + (x & 1)));
-    };
-    Piece pc;
-    while (w.next(p, pc)) {
-      alive = wait_for(bar(kQFull), pieces & 1, wait) && alive;
-      issue_s(i);
-#pragma unroll 1
-      for (int k = 0; k < pc.n; ++k, ++i) {
-        if (k + 1 < pc.n) issue_s(i + 1);
-        issue_o(i, k == 0);
+        __syncwarp();
+        if (lane < groups) {
+          if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) { bad = true; id = 0; }
+          const int in = p.bs_shift >= 0 ? n & (p.block_size - 1) : n % p.block_size;
+          copy_group(base + C::kOffRing + stage * kStageBytes + lane * 16 * p.slot_bytes, &map, q.head * p.slot_bytes, id * p.block_size + in, bar(kRingFull + stage));
+        }
+        ++issued;
+        if (++stage == C::kRing) { stage = 0; turn ^= 1; }
+        if (++tile == q.tile0 + q.n) {
+          live = w.next(p, q);
+          if (live) tile = q.tile0;
+        }
+        if (live) id = block_id();
       }
-      ++pieces;
+      if (bad) atomicOr(&g_tree_status, kStatusBadBlock);
+      // no copy may be in flight when the CTA ends, also after a wait elsewhere gave up
+      const unsigned long long t0 = global_timer_ns();
+      for (int k = max(0, issued - C::kRing); k < issued; ++k)
+        while (!mbar_try_wait(bar(kRingFull + k % C::kRing), (k / C::kRing) & 1) && global_timer_ns() - t0 < kWaitLimitNs) { }
+    } else if (warp == C::kWarpS || warp == C::kWarpO) {
+      // ============ MMA issuers: one warp for S = K Q^T, one for O += V^T P, so that neither waits for the other's operands ======
+      constexpr uint32_t idesc_s = instr_desc_f16(kKeys, NR, false, false), idesc_o = instr_desc_f16(kHeadDim, NR, true, true);
+      const bool leader = elect_one();
+      bool alive = true;
+      int i = 0, pieces = 0;
+      Piece pc;
+      if (warp == C::kWarpS) {
+        const uint64_t q_desc = smem_desc_sw128(base + C::kOffQ, 16, 1024);
+        while (w.next(p, pc)) {
+          alive = wait_for(bar(kQFull), pieces & 1, wait) && alive;
+#pragma unroll 1
+          for (int k = 0; k < pc.n; ++k, ++i) {
+            alive = wait_for(bar(kKFull + (i & 1)), (i >> 1) & 1, wait) && alive;
+            if (i >= C::kSBuffers) alive = wait_for(bar(kSEmpty + (i & (C::kSBuffers - 1))), ((i >> C::kSShift) - 1) & 1, wait) && alive;
+            __syncwarp();
+            tc_fence_after_sync();
+            const uint32_t d = tmem + C::kColS + (i & (C::kSBuffers - 1)) * NR, a = tmem + C::kColK + (i & 1) * 64;
+            if (leader && alive) {
+#pragma unroll
+              for (int term = 0; term < 2; ++term)
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                  const uint64_t q = q_desc + ((term * (NR * 256) + (ks >> 2) * (NR * 128) + (ks & 3) * 32) >> 4);
+                  if (term == 0 && ks == 0) mma_ts<false>(d, a, q, idesc_s);
+                  else mma_ts<true>(d, a + 8 * ks, q, idesc_s);
+                }
+              mma_commit(bar(kSFull + (i & (C::kSBuffers - 1))));
+              mma_commit(bar(kKEmpty + (i & 1)));
+            }
+            __syncwarp();
+          }
+          ++pieces;
+        }
+      } else {
+        const uint64_t v_desc = smem_desc_sw128(base + C::kOffV, kColBlock, 1024), p_desc = smem_desc_sw128(base + C::kOffP, kColBlock, 1024);
+        while (w.next(p, pc)) {
+#pragma unroll 1
+          for (int k = 0; k < pc.n; ++k, ++i) {
+            alive = wait_for(bar(kVFull + (i & 1)), (i >> 1) & 1, wait) && alive;
+            alive = wait_for(bar(kPFull + (i & 1)), (i >> 1) & 1, wait) && alive;
+            __syncwarp();
+            tc_fence_after_sync();
+            if (leader && alive) {
+              const uint64_t v = v_desc + (i & 1) * (kTileBytes >> 4), pt = p_desc + (C::kStreams == 2 ? (i & 1) * (kColBlock >> 4) : 0);
+#pragma unroll
+              for (int ks = 0; ks < 8; ++ks) mma_ss(tmem + C::kColO + (C::kStreams == 2 ? (i & 1) * NR : 0), v + ks * 128, pt + ks * 128, idesc_o, k < C::kStreams && ks == 0 ? 0u : 1u);
+              mma_commit(bar(kPvDone + (i & 1)));
+            }
+            __syncwarp();
+          }
+        }
+      }
+      // nothing in flight when tensor memory is released: a commit behind everything issued, waited for (with a limit) even
+      // after a wait elsewhere gave up
+      if (leader) mma_commit(bar(kDrained));
+      const unsigned long long t0 = global_timer_ns();
+      while (!mbar_try_wait(bar(kDrained), 0) && global_timer_ns() - t0 < kWaitLimitNs) { }
     }
-    // nothing in flight when tensor memory is released: a commit behind everything issued, waited for (with a limit) even
-    // after a wait elsewhere gave up
-    mma_commit(bar(kDrained));
-    const unsigned long long t0 = global_timer_ns();
-    while (!mbar_try_wait(bar(kDrained), 0) && global_timer_ns() - t0 < kWaitLimitNs) { }
   }
   __syncwarp();
   tc_fence_before_sync();
@@ -724,7 +931,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     if (wait->abort) { rec = Record{-1, 0, 3, 0}; atomicOr(&g_tree_status, kStatusWait); }
     space.rec[blockIdx.x] = rec;
   }
-  if (warp == C::kWarpMma) {
+  if (warp == C::kWarpS) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, C::kTmemCols);
   }

@@ -8,7 +8,9 @@ is below 2^-21 of the cap).  Then
   lse   off by d + 2^-22 |lse|
   out   probabilities are off by 2 d and rounded to fp16 (2^-11): (2^-11 + 2 d) sum_n p_n |v_n| in the rotated frame, which the
         rotation back spreads over the row as at most sum_d(.) / sqrt(128); the result is rounded to fp16 (2^-11 |out|, and
-        2^-25 where fp16 is subnormal)
+        2^-25 where fp16 is subnormal).  A 4-bit value row is fp16(level) * norm in the kernel and fp16(level * norm) here: either
+        rounding is off by at most half a step, 2^-11 of the value, so the two differ by at most 2^-10 |v|; where a row is
+        subnormal, by at most 2 * 2^-25 a coordinate, which spreads to less than 2^-20
   mass  every term off by 2 d of its value, and the sum of R terms by R 2^-24 of it
 """
 from __future__ import annotations
@@ -109,7 +111,8 @@ def tree_reference(c):
         d = score_bound(c, x, S)
         o = torch.einsum("htgn,hnd->htgd", p, V) @ had
         spread = torch.einsum("htgn,hnd->htgd", p, V.abs()).sum(-1, keepdim=True) / math.sqrt(128.0)
-        t = 2.0 ** -11 * o.abs() + (2.0 ** -11 + 2 * d[..., None]) * spread + 2.0 ** -25
+        rows = 2.0 ** -10 if c["v_bits"] == 4 else 0.0
+        t = 2.0 ** -11 * o.abs() + (2.0 ** -11 + rows + 2 * d[..., None]) * spread + 2.0 ** -25 + (2.0 ** -20 if rows else 0.0)
         back = lambda y: y.permute(1, 0, 2, 3).reshape(hi - lo, Hq, -1)  # noqa: E731
         out[lo:hi], tol[lo:hi] = back(o), back(t)
         lse[lo:hi], ltol[lo:hi] = back(z[..., None])[..., 0], back((d + torch.nan_to_num(z, neginf=0.0).abs() * 2.0 ** -22)[..., None])[..., 0]
