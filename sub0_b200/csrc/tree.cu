@@ -13,74 +13,12 @@ namespace cda {
 __device__ int g_tree_status = 0;
 }
 
+#include "mass_umma.cuh"
 #include "tree_umma.cuh"
 
 #include <cmath>
 
 namespace cda {
-
-// Four consecutive coordinates 4 * lane .. of one side of a slot, as the stored fp16 values.
-__device__ __forceinline__ void decode4(const uint8_t* codes, int bits, const float* cb, float norm, int lane, float (&v)[4]) {
-  int c[4];
-  if (bits == 4) {
-    const uint8_t a = codes[2 * lane], b = codes[2 * lane + 1];
-    c[0] = a >> 4; c[1] = a & 15; c[2] = b >> 4; c[3] = b & 15;
-  } else {
-    const uint8_t a = codes[lane];
-    c[0] = a >> 6; c[1] = (a >> 4) & 3; c[2] = (a >> 2) & 3; c[3] = a & 3;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = round_to_half(cb[c[i]] * norm);
-}
-
-__device__ __forceinline__ const uint8_t* slot_of(const AttendParams& p, int b, int n, int head, bool& bad) {
-  int blk = p.block_table[static_cast<int64_t>(b) * p.bt_stride + n / p.block_size];
-  if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) { bad = true; blk = 0; }
-  return p.cache + ((static_cast<int64_t>(blk) * p.block_size + n % p.block_size) * p.H_kv + head) * p.slot_bytes;
-}
-
-// Whether token t of the sequence sees key n, and the bias of the pair.
-__device__ __forceinline__ bool sees(const AttendParams& p, const SequenceView& s, int t, int n, float slope, float& bias) {
-  const int ctx = s.seq_len - s.q_len;
-  const int pos_q = ctx + depth_of(p, s.q_begin, t), pos_k = n < ctx ? n : ctx + depth_of(p, s.q_begin, n - ctx);
-  bias = slope * static_cast<float>(pos_k - pos_q);
-  if (p.window > 0 && pos_q - pos_k >= p.window) return false;
-  if (n < ctx) return true;
-  return p.tree_mask ? (static_cast<unsigned long long>(p.tree_mask[s.q_begin + t]) >> (n - ctx)) & 1ull : n - ctx <= t;
-}
-
-// One warp per (sequence, KV head, key): the rows one after another.  The key is rotated back once, so that the raw query
-// rows can be used as they are.
-__global__ void __launch_bounds__(256) mass_simple_kernel(const AttendParams p) {
-  const int lane = threadIdx.x & 31, head = blockIdx.y, b = blockIdx.z;
-  const int n = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const SequenceView s = sequence_view(p, b);
-  if (s.bad && threadIdx.x == 0 && blockIdx.x == 0 && head == 0) atomicOr(&g_tree_status, kStatusLengths);
-  if (s.q_len == 0 || n >= s.seq_len) return;
-  bool bad = false;
-  const uint8_t* slot = slot_of(p, b, n, head, bad);
-  if (bad && lane == 0) atomicOr(&g_tree_status, kStatusBadBlock);
-  float k[4];
-  decode4(slot, p.k_bits, p.cb_k, *reinterpret_cast<const float*>(slot + 16 * (p.k_bits + p.v_bits)), lane, k);
-  fht128_warp(k, lane);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) k[i] *= kRsqrtD * p.scale;
-  const float inv_cap = p.softcap > 0.f ? 1.0f / p.softcap : 0.f;
-  float sum = 0.f;
-  for (int r = 0; r < s.q_len * p.group; ++r) {
-    const int t = r / p.group, hq = head * p.group + r % p.group;
-    const int64_t row = static_cast<int64_t>(s.q_begin + t) * p.H_q + hq;
-    const float z = p.lse[row], w = p.weights ? p.weights[s.q_begin + t] : 1.0f;
-    float bias;
-    if (!sees(p, s, t, n, p.slopes ? p.slopes[hq] : 0.f, bias) || z == -INFINITY || w == 0.f) continue;
-    float q[4];
-    load_half4(p.q + row * kHeadDim + 4 * lane, q);
-    float x = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-    if (p.softcap > 0.f) x = p.softcap * soft_tanh(x * inv_cap);
-    sum += w * expf(x + bias - z);
-  }
-  if (lane == 0) p.mass[(static_cast<int64_t>(b) * p.H_kv + head) * p.mass_stride + n] += sum;
-}
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
 static int fill_params(AttendParams& p, const char* what, const void* Q, const void* kv_cache, const int32_t* block_table,
@@ -142,6 +80,21 @@ static int launch_tree(AttendParams& p, void* ws, int ctas, const CUtensorMap& m
   tru::tree_merge_kernel<NR><<<dim3(ctas, NR / 8), 256, 0, st>>>(p, ws, ctas);
   return check_launch("tree_attention: merge");
 }
+
+template <int NR>
+static int launch_mass(const AttendParams& p, const CUtensorMap& map, cudaStream_t st) {
+  using C = msu::MassCfg<NR>;
+  static bool configured[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (cudaFuncSetAttribute(msu::attention_mass_kernel<NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) != cudaSuccess)
+      return check_launch("attention_mass: shared memory opt-in");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  msu::attention_mass_kernel<NR><<<device_sm_count(-1), C::kThreads, C::kSmemBytes, st>>>(p, map);
+  return check_launch("attention_mass");
+}
 }  // namespace cda
 
 extern "C" size_t cda_b200_tree_attention_workspace_bytes(int H_q, int H_kv, int max_query_len, int device) {
@@ -201,10 +154,16 @@ extern "C" int cda_b200_attention_mass(const void* Q, const void* kv_cache, cons
   if (rc != CDA_OK) return rc;
   if (!lse || !mass) return fail(CDA_ERR_BAD_ARG, "attention_mass: null pointer");
   if (mass_stride < max_seq_len) return fail(CDA_ERR_BAD_SHAPE, "attention_mass: rows of %lld weights, max_seq_len is %d", static_cast<long long>(mass_stride), max_seq_len);
-  if (H_kv > 65535 || B > 65535) return fail(CDA_ERR_N_TOO_LARGE, "attention_mass: B %d or H_kv %d exceeds the grid limits", B, H_kv);
   p.lse = lse; p.weights = weights; p.mass = mass; p.mass_stride = mass_stride;
-  mass_simple_kernel<<<dim3((max_seq_len + 7) / 8, H_kv, B), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return check_launch("attention_mass");
+  const int64_t rows = static_cast<int64_t>(max_query_len) * p.group;
+  if ((rows + 15) / 16 * B * H_kv * ((max_seq_len + 127) / 128) > 0x7fffffffll)
+    return fail(CDA_ERR_N_TOO_LARGE, "attention_mass: %d sequences of %d new and %d old tokens are too many tiles for one call", B, max_query_len, max_seq_len);
+  CUtensorMap map;
+  if (const int map_rc = make_cache_map("attention_mass", kv_cache, H_kv, slot_bytes, static_cast<int64_t>(p.num_blocks) * block_size, slot_bytes, &map)) return map_rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // the fewest columns that hold a chunk's rows: a block of more costs the tensor cores and the exponentials as many columns,
+  // a block of fewer another pass of the K producers over all tiles
+  return rows <= 16 ? launch_mass<16>(p, map, st) : rows <= 64 ? launch_mass<64>(p, map, st) : launch_mass<128>(p, map, st);
 }
 
 namespace cda {

@@ -56,6 +56,7 @@ struct Cfg {
   // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536)
   static constexpr int kRegsSoft = 88, kRegsK = 40, kRegsV = 40, kRegsOther = 40;
   static constexpr int kRing = NR == 128 ? 2 : 4;
+  static_assert(kRing % 2 == 0, "one K group reads a stage, and so sees every phase of its barrier");
   static constexpr int kTmemCols = 512;                          // tensor memory: two K, the S, one O for each stream
   static constexpr int kColK = 0, kColS = 128, kColO = kColS + kSBuffers * NR;
   // shared memory (bytes from a 1024-aligned base)

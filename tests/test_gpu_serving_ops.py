@@ -383,3 +383,35 @@ def test_captured_and_replayed_beside_an_eager_call():
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
     assert ops.kv_status() == 0
+
+
+@pytest.mark.parametrize("B,N,group,k_bits,v_bits", [(16, 16384, 4, 4, 4), (3, 70000, 8, 4, 2), (40, 5000, 1, 2, 2)])
+def test_many_tiles_per_cta(B, N, group, k_bits, v_bits):
+    """Sizes at which every ring and buffer of the kernels wraps many times.  Each row's weights sum to one, so a sequence and KV
+    head give away as many as it has rows; a chain of one token is a decode step."""
+    from sub0_b200 import ops, synth
+    w = synth.build_decode_workload(B, N, group=group, k_bits=k_bits, v_bits=v_bits)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=DEV)
+    out, lse, ref = torch.empty_like(w.Q), torch.empty(w.Q.shape[:2], device=DEV), torch.empty_like(w.Q)
+    a = dict(cb_K=w.cb_K, block_size=16, cu_seqlens_q=cu, max_query_len=1, max_seq_len=N)
+    ops.tree_attention(w.Q, w.cache, w.block_table, w.seq_lens, out, cb_V=w.cb_V, lse=lse, **a)
+    ops.decode(w.Q, w.cache, w.block_table, w.seq_lens, ref, cb_K=w.cb_K, cb_V=w.cb_V, block_size=16, max_seq_len=N)
+    assert float(((out.float() - ref.float()).abs() / (1e-3 + 2e-3 * ref.float().abs())).max()) < 2.0
+    mass = torch.zeros(B, 8, N, device=DEV)
+    ops.attention_mass(w.Q, w.cache, w.block_table, w.seq_lens, lse, mass, **a)
+    # a sum of N terms that are off by 2^-16 of their value at most (scores of size 2^2 summed in fp32), and lse by as much
+    assert float((mass.double().sum(-1) - group).abs().max()) < group * 2.0 ** -15
+    T = 12                                                             # the same cache under longer chunks, rows in several blocks
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    Q = torch.randn(B * T, 8 * group, 128, generator=gen, device=DEV).half()
+    out, lse = torch.empty_like(Q), torch.empty(Q.shape[:2], device=DEV)
+    a.update(cu_seqlens_q=cu * T, max_query_len=T)
+    ops.tree_attention(Q, w.cache, w.block_table, w.seq_lens, out, cb_V=w.cb_V, lse=lse, **a)
+    mass.zero_()
+    ops.attention_mass(Q, w.cache, w.block_table, w.seq_lens, lse, mass, **a)
+    assert float((mass.double().sum(-1) - group * T).abs().max()) < group * T * 2.0 ** -15
+    pre = torch.empty_like(Q)
+    if group in (1, 4, 8):
+        ops.prefill_varlen(Q, w.cache, w.block_table, cu * T, w.seq_lens, pre, cb_K=w.cb_K, cb_V=w.cb_V, block_size=16, max_query_len=T, max_seq_len=N)
+        assert float(((out.float() - pre.float()).abs() / (1e-3 + 2e-3 * pre.float().abs())).max()) < 2.0
+    assert ops.kv_status() == 0
