@@ -7,10 +7,45 @@ namespace cda {
 __device__ int g_evict_status = 0;
 int tree_status(bool clear, int* value);   // tree.cu
 
+// ---- thread-block clusters ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ int4 remote_int4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ int2 remote_int2(uint32_t addr) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+
 // ---- select -----------------------------------------------------------------------------------------------------------
 // Kept of a row of n weights, when n > budget: the first `sink`, the last `recent`, and of the others the budget - sink -
-// recent largest, ties to the lower index.  The threshold is found by radix selection over the ordered bit patterns.
-constexpr int kSelectThreads = 512, kDigitBits = 11, kBins = 1 << kDigitBits;
+// recent largest, ties to the lower index.  A cluster of CTAs serves one row, a contiguous slice of it each: the slice is read
+// once and kept in shared memory as ordered keys (slices too long for it are read again in every pass); the threshold is found
+// by radix selection, 11 + 11 + 10 bits, with the CTAs' histograms added up over distributed shared memory; then every warp
+// counts and writes what it keeps of its part in ascending order.  Reading the row once is the floor (256 rows of 65536: 67 MB,
+// 10 us).
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kDigitBits = 11, kBins = 1 << kDigitBits;
+constexpr int kSliceMax = 32768;                  // keys in shared memory (128 KB)
 
 // Larger weights have larger keys; -0 counts as 0 and NaN as minus infinity, like any value below every other.
 __device__ __forceinline__ uint32_t weight_key(float x) {
@@ -19,8 +54,8 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Exclusive prefix sum of one value per thread over the CTA; returns the total through `total`.
-__device__ __forceinline__ int block_exclusive_scan(int v, int* s_warp, int& total) {
+// Exclusive prefix sum of one value per thread over the CTA.
+__device__ __forceinline__ int block_exclusive_scan(int v, int* s_warp) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
 #pragma unroll
@@ -31,91 +66,135 @@ __device__ __forceinline__ int block_exclusive_scan(int v, int* s_warp, int& tot
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
   int before = 0;
-  total = 0;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
-    if (w < warp) before += s_warp[w];
-    total += s_warp[w];
-  }
-  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelectWarps; ++w) before += w < warp ? s_warp[w] : 0;
   return before + x - v;
 }
 
 __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float* __restrict__ mass, const int32_t* __restrict__ seq_lens,
                                                                      int32_t* __restrict__ keep, int32_t* __restrict__ new_lens, int H,
-                                                                     int64_t stride, int budget, int sink, int recent) {
-  __shared__ int s_hist[kBins], s_warp[kSelectThreads / 32], s_digit, s_left;
-  const int tid = threadIdx.x, b = blockIdx.x / H;
-  const int64_t row = blockIdx.x;
+                                                                     int64_t stride, int budget, int sink, int recent, int cached) {
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  __shared__ __align__(16) int s_hist[3][kBins];
+  __shared__ int s_warp[3][kSelectWarps], s_digit, s_left;
+  __shared__ __align__(8) int2 s_count, s_part[kSelectWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int64_t row = blockIdx.x / ranks;
+  const int b = static_cast<int>(row / H);
   int n = seq_lens[b];
   if (n > stride) {
-    if (tid == 0) atomicOr(&g_evict_status, kStatusLengths);
+    if (tid == 0 && rank == 0) atomicOr(&g_evict_status, kStatusLengths);
     n = static_cast<int>(stride);
   }
   n = max(n, 0);
   int32_t* out = keep + row * budget;
-  if (tid == 0 && blockIdx.x % H == 0) new_lens[b] = min(n, budget);
-  if (n <= budget) {
-    for (int i = tid; i < budget; i += kSelectThreads) out[i] = i < n ? i : -1;
+  if (tid == 0 && rank == 0 && row % H == 0) new_lens[b] = min(n, budget);
+  const int first = rank * kSelectThreads + tid, hop = ranks * kSelectThreads;      // this thread's share of plain writes
+  if (n <= budget) {                              // (the same for all CTAs of the cluster)
+    for (int i = first; i < budget; i += hop) out[i] = i < n ? i : -1;
     return;
   }
   const float* w = mass + row * stride;
-  const int lo = sink, hi = n - recent;
-  int left = budget - sink - recent;             // how many of [lo, hi) are kept
+  const int lo = sink, hi = n - recent, wanted = budget - sink - recent;
+  for (int i = first; i < sink; i += hop) out[i] = i;
+  for (int i = first; i < recent; i += hop) out[budget - recent + i] = hi + i;
+  if (wanted == 0) return;
+  // slices of whole warps' worth, so that the order of ranks and warps is the order of the keys
+  const int slice = ((hi - lo + static_cast<int>(ranks) - 1) / static_cast<int>(ranks) + 511) / 512 * 512;
+  const int s0 = min(lo + static_cast<int>(rank) * slice, hi), s1 = min(s0 + slice, hi);
+  const bool in_shared = cached >= slice;
+  for (int i = tid; i < 3 * kBins; i += kSelectThreads) s_hist[0][i] = 0;
+  __syncthreads();
+  auto key_at = [&](int i) { return in_shared ? s_keys[i - s0] : weight_key(w[i]); };
   uint32_t prefix = 0, prefix_mask = 0;
-  if (left > 0) {
-    for (int shift = 32 - kDigitBits, bits = kDigitBits;; ) {
-      for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelectThreads) {
-        const uint32_t k = weight_key(w[i]);
-        if ((k & prefix_mask) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1 << bits) - 1)], 1);
-      }
-      __syncthreads();
-      // bins from the top: thread t owns bins kBins - 1 - 4t .. kBins - 4 - 4t
-      constexpr int kOwn = kBins / kSelectThreads;
-      int c[kOwn], sum = 0, total;
+  int left = wanted;
 #pragma unroll
-      for (int j = 0; j < kOwn; ++j) sum += c[j] = s_hist[kBins - 1 - kOwn * tid - j];
-      int above = block_exclusive_scan(sum, s_warp, total);
-#pragma unroll
-      for (int j = 0; j < kOwn; ++j) {
-        if (above < left && left <= above + c[j]) { s_digit = kBins - 1 - kOwn * tid - j; s_left = left - above; }
-        above += c[j];
+  for (int pass = 0; pass < 3; ++pass) {
+    const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+#pragma unroll 4
+    for (int i = s0 + tid; i < s1; i += kSelectThreads) {
+      uint32_t k;
+      if (pass == 0) {
+        k = weight_key(w[i]);
+        if (in_shared) s_keys[i - s0] = k;
+      } else {
+        k = key_at(i);
       }
-      __syncthreads();
-      left = s_left;
-      prefix |= static_cast<uint32_t>(s_digit) << shift;
-      prefix_mask |= ((1u << bits) - 1u) << shift;
-      __syncthreads();
-      if (shift == 0) break;
-      bits = shift < kDigitBits ? shift : kDigitBits;
-      shift -= bits;
+      if ((k & prefix_mask) == prefix) atomicAdd(&s_hist[pass][(k >> shift) & ((1 << bits) - 1)], 1);
+    }
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+    // bins from the top: thread t owns bins kBins - 4 - 4 t .. kBins - 1 - 4 t
+    static_assert(kBins == 4 * kSelectThreads, "four bins a thread");
+    const int bin0 = kBins - 4 - 4 * tid;
+    int4 c = make_int4(0, 0, 0, 0);
+    for (uint32_t r = 0; r < ranks; ++r) {
+      const int4 v = remote_int4(remote(smem_addr(&s_hist[pass][bin0]), r));
+      c.x += v.x; c.y += v.y; c.z += v.z; c.w += v.w;
+    }
+    int above = block_exclusive_scan(c.x + c.y + c.z + c.w, s_warp[pass]);
+    const int counts[4] = {c.w, c.z, c.y, c.x};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (above < left && left <= above + counts[j]) { s_digit = bin0 + 3 - j; s_left = left - above; }
+      above += counts[j];
+    }
+    __syncthreads();
+    left = s_left;
+    prefix |= static_cast<uint32_t>(s_digit) << shift;
+    prefix_mask |= ((1u << bits) - 1u) << shift;
+    __syncthreads();
+  }
+  // `prefix` is the key of the smallest kept weight, `left` how many weights equal to it are kept, lowest index first.  A warp
+  // has a contiguous part of the slice.
+  const int part = slice / kSelectWarps, p0 = min(s0 + warp * part, s1), p1 = min(p0 + part, s1);
+  int above = 0, equal = 0;
+  for (int i0 = p0; i0 < p1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t k = i < p1 ? key_at(i) : 0u;
+    above += __popc(__ballot_sync(0xffffffffu, i < p1 && k > prefix));
+    equal += __popc(__ballot_sync(0xffffffffu, i < p1 && k == prefix));
+  }
+  if (lane == 0) s_part[warp] = make_int2(above, equal);
+  __syncthreads();
+  int2 before = make_int2(0, 0), all = make_int2(0, 0);
+#pragma unroll
+  for (int u = 0; u < kSelectWarps; ++u) {
+    const int2 v = s_part[u];
+    if (u < warp) { before.x += v.x; before.y += v.y; }
+    all.x += v.x;
+    all.y += v.y;
+  }
+  if (ranks > 1) {
+    if (tid == 0) s_count = all;
+    cluster_sync();
+    for (uint32_t r = 0; r < rank; ++r) {
+      const int2 v = remote_int2(remote(smem_addr(&s_count), r));
+      before.x += v.x;
+      before.y += v.y;
     }
   }
-  // `prefix` is the key of the smallest kept weight, `left` how many weights equal to it are kept, lowest index first
-  for (int i = tid; i < sink; i += kSelectThreads) out[i] = i;
-  for (int i = tid; i < recent; i += kSelectThreads) out[budget - recent + i] = hi + i;
-  const bool any = budget - sink - recent > 0;
-  int at = sink, equal = 0;
-  for (int i0 = lo; any && i0 < hi; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < hi ? weight_key(w[i]) : 0u;
-    const bool eq = i < hi && k == prefix;
-    int eq_total, total;
-    const int rank = equal + block_exclusive_scan(eq ? 1 : 0, s_warp, eq_total);
-    const bool take = i < hi && (k > prefix || (eq && rank < left));
-    const int pos = at + block_exclusive_scan(take ? 1 : 0, s_warp, total);
-    if (take) out[pos] = i;
-    at += total;
-    equal += eq_total;
+  int at = sink + before.x + min(before.y, left), eq_seen = before.y;      // kept and equal ones in front of this warp's part
+  for (int i0 = p0; i0 < p1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t k = i < p1 ? key_at(i) : 0u, lower = (1u << lane) - 1u;
+    const uint32_t eq = __ballot_sync(0xffffffffu, i < p1 && k == prefix);
+    const bool take = i < p1 && (k > prefix || (k == prefix && eq_seen + __popc(eq & lower) < left));
+    const uint32_t taken = __ballot_sync(0xffffffffu, take);
+    if (take) out[at + __popc(taken & lower)] = i;
+    at += __popc(taken);
+    eq_seen += __popc(eq);
   }
+  if (ranks > 1) cluster_sync();                  // nobody leaves while its shared memory may be read
 }
 
 // ---- compact ----------------------------------------------------------------------------------------------------------
 // Entry i of a list moves the slot of token keep[i] to token start + i.  Every entry must point at or behind its
 // destination, so that slots may be moved in place a step at a time: what a step reads lies at or behind the first place
-// it writes, i.e. behind everything that earlier steps wrote.
-constexpr int kCompactThreads = 256;
+// it writes, i.e. behind everything that earlier steps wrote.  A cluster of CTAs shares a step: all read, all wait for one
+// another, all write.  A slot is 5 to 9 pieces of 16 bytes, read and written by neighbouring threads.
+constexpr int kCompactThreads = 256, kCompactStep = 256;      // entries of one CTA in a step
 
 struct CompactParams {
   uint8_t* cache;
@@ -129,50 +208,82 @@ struct CompactParams {
   int keep_shared;          // one list for all KV heads
 };
 
+template <int PIECES>
 __global__ void __launch_bounds__(kCompactThreads) compact_cache_kernel(const CompactParams p) {
-  const int tid = threadIdx.x, b = blockIdx.y, h = blockIdx.x;
-  const int n = min(static_cast<int64_t>(p.seq_lens[b]), static_cast<int64_t>(p.bt_stride) * p.block_size);
+  __shared__ int64_t s_from[kCompactStep], s_to[kCompactStep];  // byte offsets of the slots, -1: nothing to move
+  const int tid = threadIdx.x;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int row = blockIdx.x / ranks, b = row / p.H, h = row % p.H;
+  const int64_t room = static_cast<int64_t>(p.bt_stride) * p.block_size;
+  const int n = p.seq_lens[b] < room ? p.seq_lens[b] : static_cast<int>(room);
   const int start = p.start ? p.start[b] : 0;
   const int32_t* list = p.keep + (p.keep_shared ? static_cast<int64_t>(b) : static_cast<int64_t>(b) * p.H + h) * p.K;
   float* mass = p.mass ? p.mass + (static_cast<int64_t>(b) * p.H + h) * p.mass_stride : nullptr;
-  if (start < 0) {
-    if (tid == 0) atomicOr(&g_evict_status, kStatusKeep);
+  if (start < 0) {                                // (the same for all CTAs of the cluster)
+    if (tid == 0 && rank == 0) atomicOr(&g_evict_status, kStatusKeep);
     return;
   }
-  auto slot = [&](int t) -> uint8_t* {
+  auto slot = [&](int t) -> int64_t {
     const int blk = p.block_table[static_cast<int64_t>(b) * p.bt_stride + t / p.block_size];
-    if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) { atomicOr(&g_evict_status, kStatusBadBlock); return nullptr; }
-    return p.cache + ((static_cast<int64_t>(blk) * p.block_size + t % p.block_size) * p.H + h) * p.slot_bytes;
+    if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) { atomicOr(&g_evict_status, kStatusBadBlock); return -1; }
+    return ((static_cast<int64_t>(blk) * p.block_size + t % p.block_size) * p.H + h) * p.slot_bytes;
   };
-  for (int i0 = 0; i0 < p.K; i0 += kCompactThreads) {
-    const int i = i0 + tid;
-    uint4 row[9];
+  for (int i0 = 0; i0 < p.K; i0 += kCompactStep * static_cast<int>(ranks)) {
+    const int first = i0 + static_cast<int>(rank) * kCompactStep, i = first + tid;
+    const int count = min(kCompactStep, p.K - first);            // entries of this CTA (may be negative)
     float m = 0.f;
-    uint8_t* to = nullptr;
+    int64_t from = -1, to = -1;
     if (i < p.K) {
       const int src = list[i];
       const int64_t dst = static_cast<int64_t>(start) + i;
-      if (src >= 0 && (src < dst || src >= n)) atomicOr(&g_evict_status, kStatusKeep);
-      else if (src >= 0) {
-        const uint8_t* from = slot(src);
-        if (from && src != dst) {
-          to = slot(static_cast<int>(dst));
-          if (to)
-            for (int c = 0; c < 9; ++c)
-              if (16 * c < p.slot_bytes) row[c] = *reinterpret_cast<const uint4*>(from + 16 * c);
-        }
+      if (src >= 0 && (src < dst || src >= n)) {
+        atomicOr(&g_evict_status, kStatusKeep);
+      } else if (src >= 0) {
+        from = slot(src);
+        to = from >= 0 && src != dst ? slot(static_cast<int>(dst)) : -1;
         if (mass && src < p.mass_stride) m = mass[src];
       }
     }
+    s_from[tid] = to >= 0 ? from : -1;
+    s_to[tid] = to;
     __syncthreads();
-    if (to)
-      for (int c = 0; c < 9; ++c)
-        if (16 * c < p.slot_bytes) *reinterpret_cast<uint4*>(to + 16 * c) = row[c];
+    uint4 piece[PIECES];
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+      const int q = tid + c * kCompactThreads, e = q / PIECES;
+      if (e < count && s_from[e] >= 0) piece[c] = *reinterpret_cast<const uint4*>(p.cache + s_from[e] + 16 * (q - e * PIECES));
+    }
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+      const int q = tid + c * kCompactThreads, e = q / PIECES;
+      if (e < count && s_from[e] >= 0) *reinterpret_cast<uint4*>(p.cache + s_to[e] + 16 * (q - e * PIECES)) = piece[c];
+    }
     if (mass && i < p.K && static_cast<int64_t>(start) + i < p.mass_stride) mass[start + i] = m;
-    __syncthreads();
+    __syncthreads();                              // the offsets may be overwritten
   }
+  // all moved weights were read in front of the last step's barrier
   if (mass)
-    for (int64_t t = static_cast<int64_t>(start) + p.K + tid; t < n && t < p.mass_stride; t += kCompactThreads) mass[t] = 0.f;
+    for (int64_t t = static_cast<int64_t>(start) + p.K + rank * kCompactThreads + tid; t < n && t < p.mass_stride; t += ranks * kCompactThreads) mass[t] = 0.f;
+}
+
+// A launch in clusters of `ranks` CTAs along x.
+template <class... Params, class... Args>
+static int launch_clusters(const char* what, void (*kernel)(Params...), int rows, int ranks, int threads, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * ranks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) return check_launch(what);
+  return check_launch(what);
 }
 
 }  // namespace cda
@@ -186,8 +297,23 @@ extern "C" int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, 
   if (mass_stride > 0x7fffffffll || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "select_keys: too many weights or rows");
   if (B == 0) return CDA_OK;
   if (!mass || !seq_lens || !keep || !new_lens) return fail(CDA_ERR_BAD_ARG, "select_keys: null pointer");
-  select_keys_kernel<<<B * H_kv, kSelectThreads, 0, static_cast<cudaStream_t>(stream)>>>(mass, seq_lens, keep, new_lens, H_kv, mass_stride, budget, sink, recent);
-  return check_launch("select_keys");
+  // CTAs of a row: enough that the GPU is covered, and that a slice is short (4096 keys a CTA keep its passes below the
+  // cost of the cluster's barriers; at 65536 keys and 256 rows 8 CTAs a row take a third of the time of one)
+  const int rows = B * H_kv;
+  int ranks = 1;
+  while (ranks < 8 && mass_stride > 4096ll * ranks) ranks *= 2;
+  const int64_t slice = ((mass_stride + ranks - 1) / ranks + 511) / 512 * 512;
+  const int cached = slice <= kSliceMax ? static_cast<int>(slice) : 0;
+  static bool configured[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (cudaFuncSetAttribute(select_keys_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMax * 4) != cudaSuccess)
+      return check_launch("select_keys: shared memory opt-in");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  return launch_clusters("select_keys", select_keys_kernel, rows, ranks, kSelectThreads, static_cast<size_t>(cached) * 4, static_cast<cudaStream_t>(stream),
+                         mass, seq_lens, keep, new_lens, H_kv, mass_stride, budget, sink, recent, cached);
 }
 
 extern "C" int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table, const int32_t* seq_lens, const int32_t* keep,
@@ -197,14 +323,19 @@ extern "C" int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table
   if (slot_bytes != 144 && slot_bytes != 112 && slot_bytes != 80) return fail(CDA_ERR_BAD_SHAPE, "compact_cache: slot width %d is none of 144, 112, 80", slot_bytes);
   if (block_size <= 0 || block_size % 16) return fail(CDA_ERR_BAD_SHAPE, "compact_cache: block_size=%d is not a multiple of 16", block_size);
   if (keep_heads != 1 && keep_heads != H_kv) return fail(CDA_ERR_BAD_SHAPE, "compact_cache: keep has %d heads, the cache %d", keep_heads, H_kv);
-  if (num_slots / block_size > 0x7fffffffll || B > 65535) return fail(CDA_ERR_N_TOO_LARGE, "compact_cache: too many slots or sequences");
+  if (num_slots / block_size > 0x7fffffffll || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "compact_cache: too many slots or sequences");
   if (B == 0 || (K == 0 && !mass)) return CDA_OK;
   if (!kv_cache || !block_table || !seq_lens || (K > 0 && !keep)) return fail(CDA_ERR_BAD_ARG, "compact_cache: null pointer");
   if (!aligned16(kv_cache)) return fail(CDA_ERR_BAD_ALIGN, "compact_cache: cache must be 16-byte aligned");
   const CompactParams p{static_cast<uint8_t*>(kv_cache), block_table, seq_lens, keep, start, mass, mass_stride, B, H_kv, K, block_size,
                         block_table_stride, static_cast<int>(num_slots / block_size), slot_bytes, keep_heads == 1 ? 1 : 0};
-  compact_cache_kernel<<<dim3(H_kv, B), kCompactThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  return check_launch("compact_cache");
+  int ranks = 1;
+  while (ranks < 8 && K > kCompactStep * ranks) ranks *= 2;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rows = B * H_kv;
+  return slot_bytes == 144 ? launch_clusters("compact_cache", compact_cache_kernel<9>, rows, ranks, kCompactThreads, 0, st, p)
+       : slot_bytes == 112 ? launch_clusters("compact_cache", compact_cache_kernel<7>, rows, ranks, kCompactThreads, 0, st, p)
+                           : launch_clusters("compact_cache", compact_cache_kernel<5>, rows, ranks, kCompactThreads, 0, st, p);
 }
 
 extern "C" int cda_b200_kv_status(void) {

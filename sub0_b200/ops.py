@@ -411,11 +411,20 @@ def varlen_fwd_hadamard(Q: Tensor, k_rot: Tensor, v_rot: Tensor, output: Tensor,
 
 def _same_device(dev: torch.device, **tensors: Optional[Tensor]) -> None:
     for name, t in tensors.items():
-        if t is None:
-            continue
-        _cuda(t, name)
-        if t.device != dev:
+        if t is not None and (not isinstance(t, Tensor) or t.device != dev):
+            _cuda(t, name)
             raise ValueError(f"{name} is on {t.device}, the call on {dev}")
+
+
+def _launch(dev: torch.device, fn, *args) -> None:
+    """The C entry point on the device's current stream, with that device current."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        check(rc)
 
 
 class _AttendArgs:
@@ -484,15 +493,14 @@ def tree_attention(Q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: T
     if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.numel() != Q.shape[0] * Q.shape[1]):
         raise ValueError("lse must be a contiguous fp32 CUDA tensor of T * H_q elements")
     cbv = _cb(cb_V, a.dev)
-    with torch.cuda.device(a.dev):
-        need = tree_attention_workspace_bytes(Q.shape[1], a.cache.shape[1], int(max_query_len))
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=a.dev)
-        elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
-            raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
-        check(lib.cda_b200_tree_attention(a.Q.data_ptr(), a.cache.data_ptr(), a.bt.data_ptr(), a.cu.data_ptr(), a.sl.data_ptr(),
-                                          a.cbk.data_ptr(), cbv.data_ptr(), _ptr(a.mask), _ptr(a.slopes), output.data_ptr(),
-                                          _ptr(lse), workspace.data_ptr(), workspace.numel(), *a.head, *a.tail, _stream(a.dev)))
+    need = tree_attention_workspace_bytes(Q.shape[1], a.cache.shape[1], int(max_query_len), a.dev.index)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=a.dev)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
+    _launch(a.dev, lib.cda_b200_tree_attention, a.Q.data_ptr(), a.cache.data_ptr(), a.bt.data_ptr(), a.cu.data_ptr(), a.sl.data_ptr(),
+            a.cbk.data_ptr(), cbv.data_ptr(), _ptr(a.mask), _ptr(a.slopes), output.data_ptr(), _ptr(lse), workspace.data_ptr(),
+            workspace.numel(), *a.head, *a.tail)
 
 
 def tree_attention_workspace_bytes(H_q: int, H_kv: int, max_query_len: int, device: int = -1) -> int:
@@ -518,10 +526,9 @@ def attention_mass(Q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: T
         raise ValueError("mass must be a contiguous fp32 CUDA tensor (B, H_kv, M)")
     if weights is not None and (weights.dtype != torch.float32 or not weights.is_contiguous() or weights.numel() != Q.shape[0]):
         raise ValueError("weights must be a contiguous fp32 CUDA tensor with one element per row of Q")
-    with torch.cuda.device(a.dev):
-        check(lib.cda_b200_attention_mass(a.Q.data_ptr(), a.cache.data_ptr(), a.bt.data_ptr(), a.cu.data_ptr(), a.sl.data_ptr(),
-                                          a.cbk.data_ptr(), _ptr(a.mask), _ptr(a.slopes), lse.data_ptr(), _ptr(weights),
-                                          mass.data_ptr(), mass.shape[2], *a.head, *a.tail, _stream(a.dev)))
+    _launch(a.dev, lib.cda_b200_attention_mass, a.Q.data_ptr(), a.cache.data_ptr(), a.bt.data_ptr(), a.cu.data_ptr(), a.sl.data_ptr(),
+            a.cbk.data_ptr(), _ptr(a.mask), _ptr(a.slopes), lse.data_ptr(), _ptr(weights), mass.data_ptr(), mass.shape[2], *a.head,
+            *a.tail)
 
 
 def select_keys(mass: Tensor, seq_lens: Tensor, budget: int, *, sink: int = 0, recent: int = 0):
@@ -538,9 +545,8 @@ def select_keys(mass: Tensor, seq_lens: Tensor, budget: int, *, sink: int = 0, r
         raise ValueError("seq_lens must have one element per sequence of mass")
     keep = torch.empty(B, H, max(int(budget), 0), dtype=torch.int32, device=mass.device)
     new_lens = torch.empty(B, dtype=torch.int32, device=mass.device)
-    with torch.cuda.device(mass.device):
-        check(lib.cda_b200_select_keys(mass.data_ptr(), sl.data_ptr(), keep.data_ptr(), new_lens.data_ptr(), B, H, M, int(budget),
-                                       int(sink), int(recent), _stream(mass.device)))
+    _launch(mass.device, lib.cda_b200_select_keys, mass.data_ptr(), sl.data_ptr(), keep.data_ptr(), new_lens.data_ptr(), B, H, M,
+            int(budget), int(sink), int(recent))
     return keep, new_lens
 
 
@@ -562,10 +568,9 @@ def compact_cache(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, keep:
         raise ValueError("block_table must be (B, max_blocks), seq_lens and start (B,), keep (B, H_kv or 1, K)")
     if mass is not None and (mass.dtype != torch.float32 or not mass.is_contiguous() or mass.dim() != 3 or mass.shape[:2] != (B, H)):
         raise ValueError("mass must be a contiguous fp32 CUDA tensor (B, H_kv, M)")
-    with torch.cuda.device(dev):
-        check(lib.cda_b200_compact_cache(cache.data_ptr(), bt.data_ptr(), sl.data_ptr(), kp.data_ptr(), _ptr(st), _ptr(mass),
-                                         0 if mass is None else mass.shape[2], B, H, kp.shape[2], kp.shape[1], int(block_size),
-                                         bt.shape[1], cache.shape[0], cache.shape[2], _stream(dev)))
+    _launch(dev, lib.cda_b200_compact_cache, cache.data_ptr(), bt.data_ptr(), sl.data_ptr(), kp.data_ptr(), _ptr(st), _ptr(mass),
+            0 if mass is None else mass.shape[2], B, H, kp.shape[2], kp.shape[1], int(block_size), bt.shape[1], cache.shape[0],
+            cache.shape[2])
 
 
 def evict(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, mass: Tensor, budget: int, *, block_size: int, sink: int = 0,
