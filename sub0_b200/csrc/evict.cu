@@ -43,7 +43,7 @@ __device__ __forceinline__ int2 remote_int2(uint32_t addr) {
 // once and kept in shared memory as ordered keys (slices too long for it are read again in every pass); the threshold is found
 // by radix selection, 11 + 11 + 10 bits, with the CTAs' histograms added up over distributed shared memory; then every warp
 // counts and writes what it keeps of its part in ascending order.  Reading the row once is the floor (256 rows of 65536: 67 MB,
-// 10 us).
+// 10 us; measured 113 us, most of it the first histogram's colliding shared-memory additions and the two ordered passes).
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kDigitBits = 11, kBins = 1 << kDigitBits;
 constexpr int kSliceMax = 32768;                  // keys in shared memory (128 KB)
 
@@ -112,26 +112,39 @@ __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-#pragma unroll 4
-    for (int i = s0 + tid; i < s1; i += kSelectThreads) {
-      uint32_t k;
-      if (pass == 0) {
-        k = weight_key(w[i]);
-        if (in_shared) s_keys[i - s0] = k;
-      } else {
-        k = key_at(i);
+    constexpr int kBatch = 8;                     // keys of a thread in flight
+    for (int i0 = s0 + tid; i0 < s1; i0 += kBatch * kSelectThreads) {
+      uint32_t k[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = i0 + u * kSelectThreads;
+        if (i < s1) k[u] = pass == 0 ? __float_as_uint(w[i]) : key_at(i);
       }
-      if ((k & prefix_mask) == prefix) atomicAdd(&s_hist[pass][(k >> shift) & ((1 << bits) - 1)], 1);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = i0 + u * kSelectThreads;
+        if (i >= s1) break;
+        if (pass == 0) {
+          k[u] = weight_key(__uint_as_float(k[u]));
+          if (in_shared) s_keys[i - s0] = k[u];
+        }
+        if ((k[u] & prefix_mask) == prefix) atomicAdd(&s_hist[pass][(k[u] >> shift) & ((1 << bits) - 1)], 1);
+      }
     }
     if (ranks > 1) cluster_sync();
     else __syncthreads();
     // bins from the top: thread t owns bins kBins - 4 - 4 t .. kBins - 1 - 4 t
     static_assert(kBins == 4 * kSelectThreads, "four bins a thread");
     const int bin0 = kBins - 4 - 4 * tid;
-    int4 c = make_int4(0, 0, 0, 0);
-    for (uint32_t r = 0; r < ranks; ++r) {
-      const int4 v = remote_int4(remote(smem_addr(&s_hist[pass][bin0]), r));
-      c.x += v.x; c.y += v.y; c.z += v.z; c.w += v.w;
+    int4 c = *reinterpret_cast<const int4*>(&s_hist[pass][bin0]);
+    if (ranks > 1) {
+      int4 v[7];                                  // the other CTAs' bins, all in flight together
+#pragma unroll
+      for (uint32_t r = 1; r < 8; ++r)
+        if (r < ranks) v[r - 1] = remote_int4(remote(smem_addr(&s_hist[pass][bin0]), (rank + r) & (ranks - 1)));
+#pragma unroll
+      for (uint32_t r = 1; r < 8; ++r)
+        if (r < ranks) { c.x += v[r - 1].x; c.y += v[r - 1].y; c.z += v[r - 1].z; c.w += v[r - 1].w; }
     }
     int above = block_exclusive_scan(c.x + c.y + c.z + c.w, s_warp[pass]);
     const int counts[4] = {c.w, c.z, c.y, c.x};
@@ -297,11 +310,11 @@ extern "C" int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, 
   if (mass_stride > 0x7fffffffll || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "select_keys: too many weights or rows");
   if (B == 0) return CDA_OK;
   if (!mass || !seq_lens || !keep || !new_lens) return fail(CDA_ERR_BAD_ARG, "select_keys: null pointer");
-  // CTAs of a row: enough that the GPU is covered, and that a slice is short (4096 keys a CTA keep its passes below the
-  // cost of the cluster's barriers; at 65536 keys and 256 rows 8 CTAs a row take a third of the time of one)
-  const int rows = B * H_kv;
+  // CTAs of a row: as few as hold a slice of 16384 keys each, since adding up the histograms costs a CTA as much as some 10000
+  // keys (256 rows of 65536: 113 us with 4 CTAs a row, 215 with 8, 127 with 2); more where rows are few and the GPU idle
+  const int rows = B * H_kv, sms = device_sm_count(-1);
   int ranks = 1;
-  while (ranks < 8 && mass_stride > 4096ll * ranks) ranks *= 2;
+  while (ranks < 8 && (mass_stride > 16384ll * ranks || (mass_stride > 2048ll * ranks && rows * ranks <= sms / 2))) ranks *= 2;
   const int64_t slice = ((mass_stride + ranks - 1) / ranks + 511) / 512 * 512;
   const int cached = slice <= kSliceMax ? static_cast<int>(slice) : 0;
   static bool configured[64];
@@ -329,10 +342,11 @@ extern "C" int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table
   if (!aligned16(kv_cache)) return fail(CDA_ERR_BAD_ALIGN, "compact_cache: cache must be 16-byte aligned");
   const CompactParams p{static_cast<uint8_t*>(kv_cache), block_table, seq_lens, keep, start, mass, mass_stride, B, H_kv, K, block_size,
                         block_table_stride, static_cast<int>(num_slots / block_size), slot_bytes, keep_heads == 1 ? 1 : 0};
-  int ranks = 1;
-  while (ranks < 8 && K > kCompactStep * ranks) ranks *= 2;
+  // CTAs of a list: until each has one step, or all SMs have two (128 lists of 4096: 57 us with 4 CTAs each, 63 with 8)
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rows = B * H_kv;
+  const int rows = B * H_kv, sms = device_sm_count(-1);
+  int ranks = 1;
+  while (ranks < 8 && K > kCompactStep * ranks && rows * ranks < 2 * sms) ranks *= 2;
   return slot_bytes == 144 ? launch_clusters("compact_cache", compact_cache_kernel<9>, rows, ranks, kCompactThreads, 0, st, p)
        : slot_bytes == 112 ? launch_clusters("compact_cache", compact_cache_kernel<7>, rows, ranks, kCompactThreads, 0, st, p)
                            : launch_clusters("compact_cache", compact_cache_kernel<5>, rows, ranks, kCompactThreads, 0, st, p);

@@ -418,8 +418,8 @@ def _same_device(dev: torch.device, **tensors: Optional[Tensor]) -> None:
 
 def _launch(dev: torch.device, fn, *args) -> None:
     """The C entry point on the device's current stream, with that device current."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _stream(dev))
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _stream(dev))
@@ -443,13 +443,15 @@ def _attend_args(Q, kv_cache, block_table, seq_lens, cb_K, k_bits, v_bits, block
     _same_device(a.dev, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, cu_seqlens_q=cu_seqlens_q,
                  tree_mask=tree_mask, alibi_slopes=alibi_slopes)
     a.Q, a.cache = Q.contiguous(), _flat_cache(kv_cache)
-    a.bt, a.sl, a.cu = (_i32(t).contiguous() for t in (block_table, seq_lens, cu_seqlens_q))
+    a.bt, a.sl, a.cu = _index(block_table), _index(seq_lens), _index(cu_seqlens_q)
+    T, H_q, _ = Q.shape
+    slots, H_kv, width = a.cache.shape
     B = a.sl.numel()
     if a.bt.dim() != 2 or a.bt.shape[0] < B or a.cu.numel() != B + 1:
         raise ValueError("block_table must be (B, max_blocks), seq_lens (B,) and cu_seqlens_q (B + 1,)")
-    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.numel() != Q.shape[0]):
+    if tree_mask is not None and (tree_mask.dtype != torch.int64 or tree_mask.numel() != T):
         raise ValueError("tree_mask must hold one int64 of ancestor bits per row of Q")
-    if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.numel() != Q.shape[1]):
+    if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.numel() != H_q):
         raise ValueError("alibi_slopes must hold one fp32 slope per query head")
     if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
         raise ValueError(f"softcap must be positive and finite, got {softcap}")
@@ -459,10 +461,13 @@ def _attend_args(Q, kv_cache, block_table, seq_lens, cb_K, k_bits, v_bits, block
     a.slopes = None if alibi_slopes is None else alibi_slopes.contiguous()
     a.cbk, a.kb, a.vb = _cb(cb_K, a.dev), k_bits, v_bits
     s = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    a.head = (Q.shape[0], B, Q.shape[1], a.cache.shape[1], int(block_size), a.bt.shape[1], int(max_query_len), int(max_seq_len),
-              a.cache.shape[0], a.cache.shape[2], a.kb, a.vb)
+    a.head = (T, B, H_q, H_kv, int(block_size), a.bt.shape[1], int(max_query_len), int(max_seq_len), slots, width, k_bits, v_bits)
     a.tail = (s, 0.0 if softcap is None else float(softcap), 0 if window is None else min(int(window), 2 ** 31 - 1))
     return a
+
+
+def _index(t: Tensor) -> Tensor:
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
@@ -540,11 +545,11 @@ def select_keys(mass: Tensor, seq_lens: Tensor, budget: int, *, sink: int = 0, r
         raise ValueError("mass must be a contiguous fp32 CUDA tensor (B, H_kv, M)")
     _same_device(mass.device, seq_lens=seq_lens)
     B, H, M = mass.shape
-    sl = _i32(seq_lens).contiguous()
+    sl = _index(seq_lens)
     if sl.numel() != B:
         raise ValueError("seq_lens must have one element per sequence of mass")
-    keep = torch.empty(B, H, max(int(budget), 0), dtype=torch.int32, device=mass.device)
-    new_lens = torch.empty(B, dtype=torch.int32, device=mass.device)
+    keep = sl.new_empty((B, H, max(int(budget), 0)))
+    new_lens = sl.new_empty(B)
     _launch(mass.device, lib.cda_b200_select_keys, mass.data_ptr(), sl.data_ptr(), keep.data_ptr(), new_lens.data_ptr(), B, H, M,
             int(budget), int(sink), int(recent))
     return keep, new_lens
@@ -561,8 +566,8 @@ def compact_cache(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, keep:
     dev = kv_cache.device
     _same_device(dev, block_table=block_table, seq_lens=seq_lens, keep=keep, start=start, mass=mass)
     cache = _flat_cache(kv_cache)
-    bt, sl, kp = _i32(block_table).contiguous(), _i32(seq_lens).contiguous(), _i32(keep).contiguous()
-    st = None if start is None else _i32(start).contiguous()
+    bt, sl, kp = _index(block_table), _index(seq_lens), _index(keep)
+    st = None if start is None else _index(start)
     B, H = sl.numel(), cache.shape[1]
     if bt.dim() != 2 or bt.shape[0] < B or kp.dim() != 3 or kp.shape[0] != B or (st is not None and st.numel() != B):
         raise ValueError("block_table must be (B, max_blocks), seq_lens and start (B,), keep (B, H_kv or 1, K)")
