@@ -346,6 +346,8 @@ def _build_backend_classes():
                 raise NotImplementedError("CDA backend does not support sliding window.")
             if attn_type not in (AttentionType.DECODER,):
                 raise NotImplementedError(f"CDA backend is DECODER-only, got {attn_type}.")
+            # capped scores run on the kernel for short chunks (ops.tree_attention), decodes and prompts alike
+            self.logits_soft_cap = float(logits_soft_cap) if logits_soft_cap else None
             if self.group_size not in (4, 8):
                 raise NotImplementedError(f"CDA supports group_size in {{4, 8}}. Got group_size={self.group_size}.")
 
@@ -381,7 +383,12 @@ def _build_backend_classes():
             if md.dcp_world_size > 1:
                 if md.max_query_len > 1:
                     raise NotImplementedError("CDA decode context parallelism covers decode steps only.")
+                if self.logits_soft_cap is not None:
+                    raise NotImplementedError("CDA decode context parallelism does not cap scores.")
                 _time_call("forward_decode_dcp", lambda: self._forward_decode_dcp(q, cache, out, md))
+                return output
+            if self.logits_soft_cap is not None:
+                _time_call("forward_capped", lambda: self._forward_capped(q, cache, out, md))
                 return output
             if md.max_query_len <= 1:
                 _time_call("forward_decode", lambda: self._forward_decode(q, cache, out, md.block_table, md.seq_lens, md.max_seq_len))
@@ -416,6 +423,20 @@ def _build_backend_classes():
             if dst is not out:
                 out.copy_(dst)
 
+        def _forward_capped(self, q, cache, out, md, lse=None) -> None:
+            """A whole batch -- decodes, chunks, prompts -- with scores capped at ``logits_soft_cap``: every sequence's new
+            tokens are a causal chain over its cache."""
+            from .. import ops
+
+            flat, bs = self._flat(cache)
+            cb_K, cb_V = get_codebooks(cache.device)
+            dst = out if out.is_contiguous() else torch.empty_like(q)
+            ops.tree_attention(q.contiguous(), flat, md.block_table, md.seq_lens[:md.num_reqs], dst, cb_K=cb_K, cb_V=cb_V, block_size=bs,
+                               cu_seqlens_q=md.query_start_loc[:md.num_reqs + 1], max_query_len=int(md.max_query_len),
+                               max_seq_len=int(md.max_seq_len), scale=self.scale, softcap=self.logits_soft_cap, lse=lse)
+            if dst is not out:
+                out.copy_(dst)
+
         def forward_decode_with_lse(self, query: torch.Tensor, kv_cache: torch.Tensor, attn_metadata):
             """Decode step that also returns the log-sum-exp of the scaled scores: ``(out (n, H, 128) fp16, lse (n, H) fp32,
             natural log)`` -- what ``can_return_lse_for_decode`` promises a caller that corrects the output across ranks
@@ -430,6 +451,9 @@ def _build_backend_classes():
             cb_K, cb_V = get_codebooks(cache.device)
             out = torch.empty_like(q)
             lse = torch.empty(n, self.num_heads, dtype=torch.float32, device=q.device)
+            if self.logits_soft_cap is not None:
+                self._forward_capped(q, cache, out, md, lse)
+                return out, lse
             ops.decode(q, flat, md.block_table, md.seq_lens, out, cb_K=cb_K, cb_V=cb_V, block_size=bs, scale=self.scale,
                        max_seq_len=int(md.max_seq_len), lse=lse)
             return out, lse

@@ -415,3 +415,62 @@ def test_many_tiles_per_cta(B, N, group, k_bits, v_bits):
         ops.prefill_varlen(Q, w.cache, w.block_table, cu * T, w.seq_lens, pre, cb_K=w.cb_K, cb_V=w.cb_V, block_size=16, max_query_len=T, max_seq_len=N)
         assert float(((out.float() - pre.float()).abs() / (1e-3 + 2e-3 * pre.float().abs())).max()) < 2.0
     assert ops.kv_status() == 0
+
+
+def test_refusals_on_the_gpu():
+    """Arguments that the front end refuses before anything is launched."""
+    from sub0_b200 import ops
+    c = S.attend_case([50], [5], seed=1)
+    a, out = call_args(c), torch.empty_like(c["Q"], device=DEV)
+    pos = (on(c["Q"]), on(c["cache"]), on(c["block_table"]), on(c["seq_lens"]))
+    tree = lambda **kw: ops.tree_attention(*pos, kw.pop("out", out), cb_V=on(c["cb_V"]), **{**a, **kw})  # noqa: E731
+    for kw in (dict(softcap=0.0), dict(softcap=-1.0), dict(softcap=math.inf), dict(window=0), dict(out=out.float()), dict(out=out.cpu()),
+               dict(tree_mask=a["tree_mask"][:4]), dict(tree_mask=a["tree_mask"].int()), dict(alibi_slopes=torch.ones(3, device=DEV)),
+               dict(lse=torch.zeros(5, 8)), dict(lse=torch.zeros(5, 7, device=DEV)), dict(cu_seqlens_q=a["cu_seqlens_q"][:1]),
+               dict(workspace=torch.zeros(16, dtype=torch.uint8, device=DEV)), dict(max_seq_len=1 << 20), dict(block_size=24)):
+        with pytest.raises((ValueError, TypeError)):
+            tree(**kw)
+    with pytest.raises(NotImplementedError):
+        tree(max_query_len=65)
+    mass, lse = torch.zeros(1, 2, 50, device=DEV), torch.zeros(5, 8, device=DEV)
+    for m, z in ((mass[..., :49].contiguous(), lse), (mass.double(), lse), (mass[:, :1].contiguous(), lse), (mass, lse[:4])):
+        with pytest.raises(ValueError):
+            ops.attention_mass(*pos, z, m, **a)
+    with pytest.raises(ValueError):
+        ops.select_keys(mass, on(c["seq_lens"]), 4, sink=3, recent=2)
+    with pytest.raises(ValueError):
+        ops.compact_cache(pos[1], pos[2], pos[3], torch.zeros(1, 3, 4, dtype=torch.int32, device=DEV), block_size=16)
+    assert ops.kv_status() == 0
+
+
+def test_views_orders_and_other_index_types():
+    """Strided queries, 64-bit lengths and tables, a 4-d cache in the type vLLM allocates."""
+    from sub0_b200 import ops
+    c = S.attend_case([130, 77], [7, 3], seed=6)
+    a = call_args(c)
+    wide = torch.zeros(10, 16, 128, dtype=torch.float16, device=DEV)
+    wide[:, ::2] = on(c["Q"])
+    cache = on(c["cache"]).view(-1, 16, 2, 144).view(torch.float16)
+    out, lse = torch.empty_like(c["Q"], device=DEV), torch.empty(10, 8, device=DEV)
+    a["cu_seqlens_q"] = a["cu_seqlens_q"].long()
+    ops.tree_attention(wide[:, ::2], cache, on(c["block_table"]).long(), on(c["seq_lens"]).long(), out, cb_V=on(c["cb_V"]), lse=lse, **a)
+    check_tree(c, out, lse)
+
+
+def test_backend_caps_scores_of_decodes_and_prompts():
+    from sub0_b200.vllm_integration.cda_attn_v2 import get_backend_classes
+    from tests.test_gpu_vllm_backend import metadata, vllm_cache
+    _, Impl, _, Metadata = get_backend_classes()
+    for q_lens in ([1, 1, 45, 130], [1, 1, 1, 1]):
+        c = S.attend_case([200, 90, 300, 130], q_lens, tree=False, softcap=12.0, seed=17)
+        impl = Impl(8, 128, c["scale"], num_kv_heads=2, logits_soft_cap=12.0)
+        md, _ = metadata(Metadata, q_lens, c)
+        n = sum(q_lens)
+        out = torch.full((n + 2, 1024), float("nan"), dtype=torch.float16, device=DEV)
+        q = torch.zeros(n + 2, 1024, dtype=torch.float16, device=DEV)
+        q[:n] = on(c["Q"]).view(n, -1)
+        impl.forward(None, q, None, None, vllm_cache(c), md, output=out)
+        want, tol, wz, _ = S.tree_reference(c)
+        assert bool(((out[:n].double().cpu().view(n, 8, 128) - want).abs() <= tol).all()) and bool(out[n:].isnan().all())
+    o, z = impl.forward_decode_with_lse(q, vllm_cache(c), md)
+    check_tree(c, o, z)
