@@ -27,6 +27,7 @@ struct AttendParams {
   int64_t mass_stride;
   int64_t T;
   int B, H_q, H_kv, group, block_size, bs_shift, bt_stride, num_blocks, max_q, max_n, k_bits, v_bits, slot_bytes;
+  int side;                      // attention_mass: KV heads that neighbouring CTAs walk together
   int row_blocks;                // row blocks per sequence
   uint32_t group_magic;          // ceil(2^32 / group): row / group = umulhi(row, magic) for rows below 2^26
   float scale, softcap;          // softcap 0: none

@@ -6,7 +6,7 @@
 // With lse given there is no maximum to find and nothing to rescale, and a lane of S^T is a key: its thread adds the row's terms
 // in a fixed order, in registers, and owns the key's word of `mass` -- no atomics, no reduction across lanes.
 //
-// Warps: two weighing groups and four K producer groups of four warps (tiles in turn), one MMA issuer, one feeder.  Expanding
+// Warps: two weighing groups and four K producer groups of four warps (tiles in turn), one MMA issuer, two feeders.  Expanding
 // codes is what takes longest here (about 23 byte-permute and logic instructions for eight coordinates), hence four groups.
 // A CTA walks an equal share of all (sequence, KV head) segments' tiles; chunks of more than NR rows pass over the share's
 // tiles once per block of NR rows.
@@ -21,7 +21,7 @@ using namespace tru;
 template <int NR>
 struct MassCfg {
   static constexpr int kGroups = 2, kKGroups = 4;
-  static constexpr int kWarpK = 4 * kGroups, kWarpS = kWarpK + 4 * kKGroups, kWarpFeed = kWarpS + 1, kThreads = (kWarpFeed + 1) * 32;
+  static constexpr int kWarpK = 4 * kGroups, kWarpS = kWarpK + 4 * kKGroups, kWarpFeed = kWarpS + 1, kThreads = (kWarpFeed + kFeeders) * 32;
   static constexpr int kSBuffers = NR == 128 ? 2 : 4;
   // a multiple of the K groups: every stage is read by one group, which sees all phases of its barrier (a group that skipped one
   // would take the phase before it for the one it waits for)
@@ -38,11 +38,11 @@ struct MassCfg {
   static constexpr int kOffLevels = kOffMask + 8 * NR;
   static constexpr int kOffScan = kOffLevels + 64;
   static constexpr int kOffBar = kOffScan + 512;
-  static constexpr int kSmemBytes = kOffBar + 384 + 1024;
+  static constexpr int kSmemBytes = kOffBar + 384 + kFeeders * kFeedIdBytes + 1024;
   static_assert(kColS + kSBuffers * NR <= kTmemCols && kSmemBytes <= 232448, "one CTA");
 };
 constexpr int kMKFull = 0, kMKEmpty = 4, kMSFull = 8, kMSEmpty = 12, kMQFull = 16, kMDrained = 17, kMRingFull = 18, kMRingEmpty = 26;   // 34
-constexpr int kMOffTmem = 272, kMOffWait = 280, kMOffPlan = 296, kMOffEnd = 312, kMOffValid = 320;
+constexpr int kMOffTmem = 272, kMOffWait = 280, kMOffPlan = 296, kMOffEnd = 312, kMOffValid = 320, kMOffIds = 384;
 
 // Sequence b: the key tiles that any of its rows may see, and its row blocks.
 struct Seq { SequenceView v; int ctx, first, tiles, blocks; };
@@ -79,7 +79,7 @@ struct MassWalk {
       if (piece_n > 0) {                                        // the piece is done
         j += piece_n;
         piece_n = 0;
-        if (j == s.tiles) { j = 0; if (++h == p.H_kv) { h = 0; ++b; } }
+        if (j == s.tiles) { j = 0; if ((h += p.side) >= p.H_kv) { h %= p.side; ++b; } }
       }
       if (left <= 0 || b >= B) return false;
       s = seq_of<NR>(p, b);
@@ -92,7 +92,10 @@ struct MassWalk {
   }
 };
 
-// Share of this CTA on the line of all segments, a tile of a sequence of several row blocks being as long as their number.
+// Share of this CTA on the line of all segments, a tile of a sequence of several row blocks being as long as their number.  `side`
+// neighbouring CTAs (the largest divisor of H_kv up to 8) walk the same share, each for its own KV head: the heads of a token lie
+// side by side, in pieces that are no whole memory lines, so they have to be read at about the same time.  (With the heads one
+// after the other on the line, 32 x 16k keys of 8 heads read 1.33 GB from memory, at 5.9 TB/s, where the slots hold 0.60 GB.)
 template <int NR, int THREADS>
 __device__ __forceinline__ void find_mass_share(const AttendParams& p, longlong2* s_scan, int* s_plan, int* s_end) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -117,16 +120,18 @@ __device__ __forceinline__ void find_mass_share(const AttendParams& p, longlong2
     if (w < warp) { tiles_before += s_scan[w].x; at += s_scan[w].y; }
     all += s_scan[w].y;
   }
-  at *= p.H_kv;
-  const long long line = all * p.H_kv, busy = line < gridDim.x ? line : gridDim.x, cta = blockIdx.x < busy ? blockIdx.x : busy;
+  const int turns = p.H_kv / p.side;                            // heads that a CTA's segments of a sequence are of
+  const unsigned teams = gridDim.x / p.side, team = blockIdx.x / p.side;
+  at *= turns;
+  const long long line = all * turns, busy = line < teams ? line : teams, cta = team < busy ? team : busy;
   const long long lo = busy ? line * cta / busy : 0, hi = cta < busy ? line * (cta + 1) / busy : lo;
   if (tid == 0) s_plan[3] = *s_end = 0;
   __syncthreads();
-  long long real = tiles_before * p.H_kv;
+  long long real = tiles_before * turns;
   for (int b = b0; hi > lo && b < b1 && at < hi; ++b) {
     const Seq s = seq_of<NR>(p, b);
     if (s.tiles == 0) continue;
-    const long long one = static_cast<long long>(s.tiles) * s.blocks + kPieceCost, next = at + one * p.H_kv;
+    const long long one = static_cast<long long>(s.tiles) * s.blocks + kPieceCost, next = at + one * turns;
     const auto tile_of = [&](long long off) { return static_cast<int>(off > kPieceCost ? (off - kPieceCost) / s.blocks : 0); };
     if (at <= lo && lo < next) {
       s_plan[0] = b; s_plan[1] = static_cast<int>((lo - at) / one); s_plan[2] = tile_of((lo - at) % one);
@@ -134,7 +139,7 @@ __device__ __forceinline__ void find_mass_share(const AttendParams& p, longlong2
     }
     if (at < hi && hi <= next) *s_end = static_cast<int>(real + (hi - at) / one * s.tiles + tile_of((hi - at) % one));
     at = next;
-    real += static_cast<long long>(s.tiles) * p.H_kv;
+    real += static_cast<long long>(s.tiles) * turns;
   }
   __syncthreads();
   if (tid == 0) s_plan[3] = *s_end - s_plan[3];
@@ -175,7 +180,7 @@ __global__ void __launch_bounds__(MassCfg<NR>::kThreads, 1) attention_mass_kerne
   tc_fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + C::kOffBar + kMOffTmem);
   MassWalk<NR> w;
-  w.b = s_plan[0]; w.h = s_plan[1]; w.j = s_plan[2]; w.left = s_plan[3]; w.B = p.B; w.piece_n = 0; w.rb = 0; w.s.blocks = 0;
+  w.b = s_plan[0]; w.h = s_plan[1] * p.side + blockIdx.x % p.side; w.j = s_plan[2]; w.left = s_plan[3]; w.B = p.B; w.piece_n = 0; w.rb = 0; w.s.blocks = 0;
   Sub q;
 
   if (warp < C::kWarpK) {
@@ -378,41 +383,12 @@ __global__ void __launch_bounds__(MassCfg<NR>::kThreads, 1) attention_mass_kerne
     const unsigned long long t0 = global_timer_ns();
     while (!mbar_try_wait(bar(kMDrained), 0) && global_timer_ns() - t0 < kWaitLimitNs) { }
   } else {
-    // ============ feeder: one lane per 16-token group of a tile; block ids are read one tile ahead ==============================
-    bool live = w.next(p, q), bad = false, alive = true;
-    int tile = live ? q.tile0 : 0, issued = 0;
-    auto block_id = [&]() {
-      const int n = min(tile * kKeys + 16 * (lane & 7), q.s.v.seq_len - 1);
-      return __ldg(p.block_table + static_cast<int64_t>(q.b) * p.bt_stride + (p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size));
-    };
-    int id = live ? block_id() : 0;
-#pragma unroll 1
-    while (live && alive) {
-      const int stage = issued % C::kRing;
-      if (issued >= C::kRing) alive = wait_for(bar(kMRingEmpty + stage), (issued / C::kRing - 1) & 1, wait);
-      if (!__all_sync(0xffffffffu, alive)) break;
-      const int left = q.s.v.seq_len - tile * kKeys, groups = min(8, (left + 15) >> 4), n = tile * kKeys + 16 * lane;
-      if (lane == 0) {
-        *reinterpret_cast<volatile int*>(sm + C::kOffBar + kMOffValid + 4 * stage) = min(left, kKeys);
-        expect_bytes(bar(kMRingFull + stage), groups * 16 * p.slot_bytes);
-      }
-      __syncwarp();
-      if (lane < groups) {
-        if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) { bad = true; id = 0; }
-        const int in = p.bs_shift >= 0 ? n & (p.block_size - 1) : n % p.block_size;
-        copy_group(base + C::kOffRing + stage * kStageBytes + lane * 16 * p.slot_bytes, &map, q.head * p.slot_bytes, id * p.block_size + in, bar(kMRingFull + stage));
-      }
-      ++issued;
-      if (++tile == q.tile0 + q.n) {
-        live = w.next(p, q);
-        if (live) tile = q.tile0;
-      }
-      if (live) id = block_id();
-    }
-    if (bad) atomicOr(&g_tree_status, kStatusBadBlock);
-    const unsigned long long t0 = global_timer_ns();            // no copy may be in flight when the CTA ends
-    for (int k = max(0, issued - C::kRing); k < issued; ++k)
-      while (!mbar_try_wait(bar(kMRingFull + k % C::kRing), (k / C::kRing) & 1) && global_timer_ns() - t0 < kWaitLimitNs) { }
+    feed_ring<C::kRing>(p, &map, [&](Feed& f) {
+      if (!w.next(p, q)) return false;
+      f = Feed{q.b, q.head, q.s.v.seq_len, q.tile0, q.n};
+      return true;
+    }, warp - C::kWarpFeed, base + C::kOffRing, bar(kMRingFull), bar(kMRingEmpty),
+        reinterpret_cast<volatile int*>(sm + C::kOffBar + kMOffValid), reinterpret_cast<int32_t*>(sm + C::kOffBar + kMOffIds), wait);
   }
   __syncwarp();
   tc_fence_before_sync();

@@ -155,6 +155,7 @@ extern "C" int cda_b200_attention_mass(const void* Q, const void* kv_cache, cons
   if (!lse || !mass) return fail(CDA_ERR_BAD_ARG, "attention_mass: null pointer");
   if (mass_stride < max_seq_len) return fail(CDA_ERR_BAD_SHAPE, "attention_mass: rows of %lld weights, max_seq_len is %d", static_cast<long long>(mass_stride), max_seq_len);
   p.lse = lse; p.weights = weights; p.mass = mass; p.mass_stride = mass_stride;
+  for (p.side = H_kv < 8 ? H_kv : 8; H_kv % p.side; ) --p.side;
   const int64_t rows = static_cast<int64_t>(max_query_len) * p.group;
   if ((rows + 15) / 16 * B * H_kv * ((max_seq_len + 127) / 128) > 0x7fffffffll)
     return fail(CDA_ERR_N_TOO_LARGE, "attention_mass: %d sequences of %d new and %d old tokens are too many tiles for one call", B, max_query_len, max_seq_len);

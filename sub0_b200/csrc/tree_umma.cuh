@@ -10,7 +10,7 @@
 // since a lane is a key, the K producers hand their expanded rows to the tensor core through tensor memory, lane by lane,
 // without a pass through shared memory.
 //
-// Warps: four softmax groups, two K producer groups and one V producer group of four warps each (a thread is a key), two MMA issuers, and a feeder that brings the slots into a ring in shared memory with tensor-map copies of
+// Warps: four softmax groups, two K producer groups and one V producer group of four warps each (a thread is a key), two MMA issuers, and two feeders that bring the slots into a ring in shared memory with tensor-map copies of
 // 16 slots of one head.  In a group that waits, one warp polls and the others are parked on a named barrier, where they take no
 // issue slots (27 polling warps spent a third of the kernel's instructions).
 // A CTA walks an equal share of all (sequence, row block, KV head) segments' tiles; a segment that starts and ends in one CTA
@@ -38,7 +38,11 @@ constexpr int kRowShift = 5;                     // look-up (32 copies: 32 KB, o
 constexpr uint32_t kRowMask = 255u << kRowShift; // a table row is 4 * kCopies bytes
 constexpr float kNoRef = 1.0e30f;                // stored negated reference of a row without one: any score exceeds it
 constexpr float kSafe = 14.0f;
+constexpr int kFeeders = 2, kFeedIdBytes = 256;   // block ids: two chunks of four tiles for each feeder
 constexpr int kPieceCost = 3;                    // what starting and ending a piece costs, in tiles (the share of a CTA counts it)
+
+constexpr int kKFull = 0, kKEmpty = 2, kVFull = 4, kSFull = 6, kSEmpty = 10, kPFull = 14, kPvDone = 16, kQFull = 18, kDrained = 19, kRingFull = 20, kRingEmpty = 24;
+constexpr int kOffTmemAddr = 224, kOffWait = 232, kOffPlan = 248, kOffPlanEnd = 264, kOffValid = 272, kOffIds = 320;   // inside kOffBar; valid: keys of each ring stage
 
 template <int NR>
 struct Cfg {
@@ -52,7 +56,7 @@ struct Cfg {
   static constexpr int kChunk = kOwn < 16 ? kOwn : 16;           // so many at a time
   static constexpr int kSoftWarps = 16, kProducerWarps = 12;     // four softmax groups; two K groups, one V group
   static constexpr int kWarpK = kSoftWarps, kWarpV = kWarpK + 8, kWarpS = kWarpV + 4, kWarpO = kWarpS + 1, kWarpFeed = kWarpO + 1;
-  static constexpr int kThreads = (kWarpFeed + 2) * 32;          // the last warp is idle: registers are handed out by four warps
+  static constexpr int kThreads = (kWarpFeed + kFeeders) * 32;   // 32 warps: registers are handed out by four warps
   // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536)
   static constexpr int kRegsSoft = 88, kRegsK = 40, kRegsV = 40, kRegsOther = 40;
   static constexpr int kRing = NR == 128 ? 2 : 4;
@@ -73,12 +77,10 @@ struct Cfg {
   static constexpr int kOffVal = kOffCmb + 16 * NR;               // 8 tiles x 128 floats: log2 of the value norms
   static constexpr int kOffLevels = kOffVal + 4096;               // 2 x 16 floats
   static constexpr int kOffBar = kOffLevels + 128;                // barriers, TMEM address, wait state, plan
-  static constexpr int kSmemBytes = kOffBar + 320 + 1024;
+  static constexpr int kSmemBytes = kOffBar + kOffIds + kFeeders * kFeedIdBytes + 1024;
   static_assert(kSmemBytes <= 232448, "one CTA's shared memory");
   static_assert(8 * (kThreads / 32) <= 1024 * kCopies, "the prologue's scan words fit the table's");
 };
-constexpr int kKFull = 0, kKEmpty = 2, kVFull = 4, kSFull = 6, kSEmpty = 10, kPFull = 14, kPvDone = 16, kQFull = 18, kDrained = 19, kRingFull = 20, kRingEmpty = 24;
-constexpr int kOffTmemAddr = 224, kOffWait = 232, kOffPlan = 248, kOffPlanEnd = 264, kOffValid = 272;   // inside kOffBar; valid: keys of each ring stage
 
 // ---- shared memory access -----------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -329,6 +331,72 @@ __device__ __forceinline__ void copy_group(uint32_t dst, const CUtensorMap* map,
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
                : "memory");
+}
+
+// Tiles [tile0, tile0 + n) of a piece, as the feeders see it.
+struct Feed { int b, head, seq_len, tile0, n; };
+// A feeder warp: copies every kFeeders-th tile of the CTA's walk to the ring, one lane per 16-token group.  A lane's copy takes
+// about 90 cycles to issue, eight of them and the stage's bookkeeping 1250: two warps, or the ring is never full.  Block ids
+// come four tiles at a time (one a lane), asynchronously into shared memory while the chunk before them is copied -- a load into a
+// register was waited for at once, 2000 cycles under load -- across the end of a piece too.  Each feeder sees every phase of its
+// stages' barriers.
+template <int RING, class Next>
+__device__ __forceinline__ void feed_ring(const AttendParams& p, const CUtensorMap* map, Next next, int which, uint32_t ring, uint32_t full, uint32_t empty,
+                                          volatile int* valid, int32_t* ids, volatile WaitState* wait) {
+  static_assert(RING % kFeeders == 0, "one feeder for each stage");
+  const int lane = threadIdx.x & 31;
+  const uint32_t ids_at = smem_addr(ids) + kFeedIdBytes * which + 4 * lane;
+  auto fetch_ids = [&](const Feed& f, int k, int half) {        // tokens past the end: the last one's block
+    const int n = min((f.tile0 + k) * kKeys + 16 * lane, f.seq_len - 1);
+    const int32_t* from = p.block_table + static_cast<int64_t>(f.b) * p.bt_stride + (p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ids_at + 128 * half), "l"(from) : "memory");
+  };
+  Feed f, after;
+  bool live = next(f), bad = false, alive = true;
+  int issued = 0, half = 0, k = 0;
+  if (live) fetch_ids(f, 0, 0);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  while (live && alive) {
+    const bool more = k + 4 < f.n;
+    if (more) fetch_ids(f, k + 4, half ^ 1);
+    else {
+      live = next(after);
+      if (live) fetch_ids(after, 0, half ^ 1);
+    }
+    asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;" ::: "memory");
+    uint32_t id4;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(id4) : "r"(ids_at + 128 * half) : "memory");
+#pragma unroll 1
+    for (const int end = min(k + 4, f.n), k0 = k; k < end; ++k, ++issued) {
+      if (issued % kFeeders != which) continue;
+      const int tile = f.tile0 + k, stage = issued % RING, turn = issued / RING;
+      if (turn > 0) alive = wait_for(empty + 8 * stage, (turn - 1) & 1, wait);
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive) break;
+      const int left = f.seq_len - tile * kKeys, groups = min(8, (left + 15) >> 4), n = tile * kKeys + 16 * (lane & 7);
+      int id = static_cast<int>(__shfl_sync(0xffffffffu, id4, 8 * (k - k0) + (lane & 7)));
+      if (lane == 0) {
+        valid[stage] = min(left, kKeys);
+        expect_bytes(full + 8 * stage, groups * 16 * p.slot_bytes);
+      }
+      __syncwarp();
+      if (lane < groups) {
+        if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) { bad = true; id = 0; }
+        const int in = p.bs_shift >= 0 ? n & (p.block_size - 1) : n % p.block_size;
+        copy_group(ring + stage * kStageBytes + lane * 16 * p.slot_bytes, map, f.head * p.slot_bytes, id * p.block_size + in, full + 8 * stage);
+      }
+      __syncwarp();
+    }
+    half ^= 1;
+    if (!more) { f = after; k = 0; }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (bad) atomicOr(&g_tree_status, kStatusBadBlock);
+  // no copy may be in flight when the CTA ends, also after a wait elsewhere gave up
+  const unsigned long long t0 = global_timer_ns();
+  for (int i = max(0, issued - RING); i < issued; ++i)
+    if (i % kFeeders == which)
+      while (!mbar_try_wait(full + 8 * (i % RING), (i / RING) & 1) && global_timer_ns() - t0 < kWaitLimitNs) { }
 }
 
 template <int NR>
@@ -827,44 +895,14 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     }
   } else {
     lower_registers<C::kRegsOther>();
-    if (warp == C::kWarpFeed) {
-      // ============ feeder: one lane per 16-token group of a tile; block ids are read one tile ahead ============================
-      Piece q;
-      bool live = w.next(p, q), bad = false, alive = true;
-      int tile = live ? q.tile0 : 0, stage = 0, turn = 0, issued = 0;
-      auto block_id = [&]() {
-        const int n = min(tile * kKeys + 16 * (lane & 7), q.x.seq_len - 1);
-        return __ldg(p.block_table + static_cast<int64_t>(q.x.b) * p.bt_stride + (p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size));
-      };
-      int id = live ? block_id() : 0;
-#pragma unroll 1
-      while (live && alive) {
-        if (issued >= C::kRing) alive = wait_for(bar(kRingEmpty + stage), turn ^ 1, wait);
-        if (!__all_sync(0xffffffffu, alive)) break;
-        const int left = q.x.seq_len - tile * kKeys, groups = min(8, (left + 15) >> 4), n = tile * kKeys + 16 * lane;
-        if (lane == 0) {
-          *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage) = min(left, kKeys);
-          expect_bytes(bar(kRingFull + stage), groups * 16 * p.slot_bytes);
-        }
-        __syncwarp();
-        if (lane < groups) {
-          if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_blocks)) { bad = true; id = 0; }
-          const int in = p.bs_shift >= 0 ? n & (p.block_size - 1) : n % p.block_size;
-          copy_group(base + C::kOffRing + stage * kStageBytes + lane * 16 * p.slot_bytes, &map, q.head * p.slot_bytes, id * p.block_size + in, bar(kRingFull + stage));
-        }
-        ++issued;
-        if (++stage == C::kRing) { stage = 0; turn ^= 1; }
-        if (++tile == q.tile0 + q.n) {
-          live = w.next(p, q);
-          if (live) tile = q.tile0;
-        }
-        if (live) id = block_id();
-      }
-      if (bad) atomicOr(&g_tree_status, kStatusBadBlock);
-      // no copy may be in flight when the CTA ends, also after a wait elsewhere gave up
-      const unsigned long long t0 = global_timer_ns();
-      for (int k = max(0, issued - C::kRing); k < issued; ++k)
-        while (!mbar_try_wait(bar(kRingFull + k % C::kRing), (k / C::kRing) & 1) && global_timer_ns() - t0 < kWaitLimitNs) { }
+    if (warp >= C::kWarpFeed) {
+      feed_ring<C::kRing>(p, &map, [&](Feed& f) {
+        Piece q;
+        if (!w.next(p, q)) return false;
+        f = Feed{q.x.b, q.head, q.x.seq_len, q.tile0, q.n};
+        return true;
+      }, warp - C::kWarpFeed, base + C::kOffRing, bar(kRingFull), bar(kRingEmpty),
+          reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid), reinterpret_cast<int32_t*>(sm + C::kOffBar + kOffIds), wait);
     } else if (warp == C::kWarpS || warp == C::kWarpO) {
       // ============ MMA issuers: one warp for S = K Q^T, one for O += V^T P, so that neither waits for the other's operands ======
       constexpr uint32_t idesc_s = instr_desc_f16(kKeys, NR, false, false), idesc_o = instr_desc_f16(kHeadDim, NR, true, true);
