@@ -18,6 +18,8 @@ namespace msu {
 
 using namespace tru;
 
+constexpr int kMassPieceCost = 3;                // what a new piece costs, in tiles
+
 template <int NR>
 struct MassCfg {
   static constexpr int kGroups = 2, kKGroups = 4;
@@ -104,7 +106,7 @@ __device__ __forceinline__ void find_mass_share(const AttendParams& p, longlong2
   for (int b = b0; b < b1; ++b) {
     const Seq s = seq_of<NR>(p, b);
     tiles += s.tiles;
-    len += s.tiles > 0 ? static_cast<long long>(s.tiles) * s.blocks + kPieceCost : 0;
+    len += s.tiles > 0 ? static_cast<long long>(s.tiles) * s.blocks + kMassPieceCost : 0;
     if (blockIdx.x == 0 && s.v.bad) atomicOr(&g_tree_status, kStatusLengths);
   }
   long long x = tiles, y = len;
@@ -131,8 +133,8 @@ __device__ __forceinline__ void find_mass_share(const AttendParams& p, longlong2
   for (int b = b0; hi > lo && b < b1 && at < hi; ++b) {
     const Seq s = seq_of<NR>(p, b);
     if (s.tiles == 0) continue;
-    const long long one = static_cast<long long>(s.tiles) * s.blocks + kPieceCost, next = at + one * turns;
-    const auto tile_of = [&](long long off) { return static_cast<int>(off > kPieceCost ? (off - kPieceCost) / s.blocks : 0); };
+    const long long one = static_cast<long long>(s.tiles) * s.blocks + kMassPieceCost, next = at + one * turns;
+    const auto tile_of = [&](long long off) { return static_cast<int>(off > kMassPieceCost ? (off - kMassPieceCost) / s.blocks : 0); };
     if (at <= lo && lo < next) {
       s_plan[0] = b; s_plan[1] = static_cast<int>((lo - at) / one); s_plan[2] = tile_of((lo - at) % one);
       s_plan[3] = static_cast<int>(real + static_cast<long long>(s_plan[1]) * s.tiles + s_plan[2]);

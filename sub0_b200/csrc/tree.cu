@@ -77,8 +77,18 @@ static int launch_tree(AttendParams& p, void* ws, int ctas, const CUtensorMap& m
   tru::tree_attention_kernel<NR><<<ctas, tru::Cfg<NR>::kThreads, tru::Cfg<NR>::kSmemBytes, st>>>(p, ws, map);
   const int rc = check_launch("tree_attention");
   if (rc != CDA_OK) return rc;
-  tru::tree_merge_kernel<NR><<<dim3(ctas, NR / 8), 256, 0, st>>>(p, ws, ctas);
-  return check_launch("tree_attention: merge");
+  // the merge starts before the first kernel ends (its blocks wait there): its launch costs no time of its own
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, NR / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, tru::tree_merge_kernel<NR>, const_cast<const AttendParams&>(p), ws, ctas) != cudaSuccess) return check_launch("tree_attention: merge");
+  return CDA_OK;
 }
 
 template <int NR>

@@ -39,7 +39,10 @@ constexpr uint32_t kRowMask = 255u << kRowShift; // a table row is 4 * kCopies b
 constexpr float kNoRef = 1.0e30f;                // stored negated reference of a row without one: any score exceeds it
 constexpr float kSafe = 14.0f;
 constexpr int kFeeders = 2, kFeedIdBytes = 256;   // block ids: two chunks of four tiles for each feeder
-constexpr int kPieceCost = 3;                    // what starting and ending a piece costs, in tiles (the share of a CTA counts it)
+// What starting and ending a piece costs, in tiles (the share of a CTA counts it): preparing and writing out few rows is quick.
+// Chains of 16 rows: 61 us with 2, 66 with 5; trees of 64 rows: 143 us with 7, 158 with 3.
+template <int NR>
+constexpr int kPieceCost = NR == 16 ? 2 : 7;
 
 constexpr int kKFull = 0, kKEmpty = 2, kVFull = 4, kSFull = 6, kSEmpty = 10, kPFull = 14, kPvDone = 16, kQFull = 18, kDrained = 19, kRingFull = 20, kRingEmpty = 24;
 constexpr int kOffTmemAddr = 224, kOffWait = 232, kOffPlan = 248, kOffPlanEnd = 264, kOffValid = 272, kOffIds = 320;   // inside kOffBar; valid: keys of each ring stage
@@ -76,7 +79,8 @@ struct Cfg {
   static constexpr int kOffCmb = kOffMax + 16 * NR * kStreams;               // 4 x NR floats: how the groups' results are put together
   static constexpr int kOffVal = kOffCmb + 16 * NR;               // 8 tiles x 128 floats: log2 of the value norms
   static constexpr int kOffLevels = kOffVal + 4096;               // 2 x 16 floats
-  static constexpr int kOffBar = kOffLevels + 128;                // barriers, TMEM address, wait state, plan
+  static constexpr int kOffBox = kOffLevels + 128;               // two boxes for each softmax warp
+  static constexpr int kOffBar = kOffBox + 128 * kSoftWarps;                // barriers, TMEM address, wait state, plan
   static constexpr int kSmemBytes = kOffBar + kOffIds + kFeeders * kFeedIdBytes + 1024;
   static_assert(kSmemBytes <= 232448, "one CTA's shared memory");
   static_assert(8 * (kThreads / 32) <= 1024 * kCopies, "the prologue's scan words fit the table's");
@@ -130,7 +134,7 @@ __device__ __forceinline__ bool group_any(int group, bool mine) {
 }
 __device__ __forceinline__ float warp_max(float x) {
   float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
   return r;
 }
 template <int N>
@@ -224,6 +228,9 @@ __device__ __forceinline__ Entry entry_of(const AttendParams& p, int e) {
   return x;
 }
 struct Piece { Entry x; int e, head, tile0, n; bool starts, ends; };
+// What a softmax warp needs of a piece at its start and end, and where its walk stands, in shared memory (a box for each warp):
+// held in registers they were spilled, and every start and end of a piece waited for L2 (1024 threads' stacks fit no L1).
+struct Box { int rb, q_begin, q_len, ctx, seq_len, t0, head, e, tile0, n, edges, walk_e, walk_h, walk_j, walk_left, pad; };
 template <int NR>
 struct Walk {
   int e, h, j, left, entries;
@@ -283,33 +290,31 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int2* s_scan, 
   }
   if (lane == 31) s_scan[warp] = make_int2(x, y);
   __syncthreads();
-  int tiles_before = x - tiles, used_before = y - used, all_tiles = 0, all_used = 0;
-  for (int w = 0; w < THREADS / 32; ++w) {
-    const int2 s = s_scan[w];
-    if (w < warp) { tiles_before += s.x; used_before += s.y; }
-    all_tiles += s.x;
-    all_used += s.y;
-  }
-  const int64_t line = static_cast<int64_t>(all_tiles + kPieceCost * all_used) * p.H_kv;
+  static_assert(THREADS == 1024, "a lane for every warp's total");
+  const int2 s = s_scan[lane];
+  const int tiles_before = x - tiles + __reduce_add_sync(0xffffffffu, lane < warp ? s.x : 0);
+  const int used_before = y - used + __reduce_add_sync(0xffffffffu, lane < warp ? s.y : 0);
+  const int all_tiles = __reduce_add_sync(0xffffffffu, s.x), all_used = __reduce_add_sync(0xffffffffu, s.y);
+  const int64_t line = static_cast<int64_t>(all_tiles + kPieceCost<NR> * all_used) * p.H_kv;
   const int busy = static_cast<int>(line < gridDim.x ? line : gridDim.x), cta = min(static_cast<int>(blockIdx.x), busy);
   const int64_t lo = busy ? line * cta / busy : 0, hi = cta < busy ? line * (cta + 1) / busy : lo;
   if (tid == 0) s_plan[3] = *s_end = 0;
   __syncthreads();
-  int64_t at = static_cast<int64_t>(tiles_before + kPieceCost * used_before) * p.H_kv;
-  const int64_t mine = static_cast<int64_t>(tiles + kPieceCost * used) * p.H_kv;
+  int64_t at = static_cast<int64_t>(tiles_before + kPieceCost<NR> * used_before) * p.H_kv;
+  const int64_t mine = static_cast<int64_t>(tiles + kPieceCost<NR> * used) * p.H_kv;
   if (hi > lo && hi > at && lo < at + mine) {                    // the line's positions lo or hi - 1 may lie in these entries
     int real = tiles_before * p.H_kv;
     for (int e = e0; e < e1; ++e) {
-      const int n = entry_of<NR>(p, e).tiles, len = n + kPieceCost;
+      const int n = entry_of<NR>(p, e).tiles, len = n + kPieceCost<NR>;
       if (n == 0) continue;
       const int64_t next = at + static_cast<int64_t>(len) * p.H_kv;
       if (at <= lo && lo < next) {
-        const int h = static_cast<int>(lo - at) / len, j = max(static_cast<int>(lo - at) % len - kPieceCost, 0);
+        const int h = static_cast<int>(lo - at) / len, j = max(static_cast<int>(lo - at) % len - kPieceCost<NR>, 0);
         s_plan[0] = e; s_plan[1] = h; s_plan[2] = j;
         s_plan[3] = real + h * n + j;
       }
       if (at < hi && hi <= next) {
-        const int h = static_cast<int>(hi - at) / len, j = max(static_cast<int>(hi - at) % len - kPieceCost, 0);
+        const int h = static_cast<int>(hi - at) / len, j = max(static_cast<int>(hi - at) % len - kPieceCost<NR>, 0);
         *s_end = real + h * n + j;
       }
       at = next;
@@ -415,6 +420,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
 
   find_share<NR, C::kThreads>(p, reinterpret_cast<int2*>(sm + C::kOffTab), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kOffPlanEnd));
   const int total = s_plan[3];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may take its places; it waits for this kernel's end
   if (total == 0) {
     if (tid == 0) space.rec[blockIdx.x] = Record{-1, 0, 0, 0};
     return;
@@ -458,48 +464,65 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t fac_a = base + C::kOffFac + 4 * C::kCols * group, max_a = base + C::kOffMax + 16 * C::kCols * group;
     const float kf = p.scale * kLog2e, cap2 = p.softcap * kLog2e, inv_cap = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
-    constexpr int kRowsWarp = C::kOwn / 4;
-    auto place = [&](const Piece& q, int r, int& t) {           // row r of the block: its token, and its index in (T, H_q)
-      const int row = q.x.rb * NR + r;
+    constexpr int kRowsWarp = C::kOwn / 4, kPair = kRowsWarp < 2 ? 1 : 2;
+    volatile Box* boxes = reinterpret_cast<volatile Box*>(sm + C::kOffBox) + 2 * warp;   // the piece in work, the one after it
+    auto next_piece = [&](int from, int into) {                 // the walk goes on from the state in one box; the piece into the other
+      volatile Box &a = boxes[from], &b = boxes[into];
+      Walk<NR> at{a.walk_e, a.walk_h, a.walk_j, a.walk_left, p.B * p.row_blocks};
+      Piece q;
+      const bool any = at.next(p, q);
+      __syncwarp();
+      if (any && lane == 0) {
+        b.rb = q.x.rb; b.q_begin = q.x.q_begin; b.q_len = q.x.q_len; b.ctx = q.x.ctx; b.seq_len = q.x.seq_len; b.t0 = q.x.t0;
+        b.head = q.head; b.e = q.e; b.tile0 = q.tile0; b.n = q.n; b.edges = (q.starts ? 2 : 0) + (q.ends ? 1 : 0);
+        b.walk_e = at.e; b.walk_h = at.h; b.walk_j = at.j; b.walk_left = at.left;
+      }
+      __syncwarp();
+      return any;
+    };
+    auto place = [&](const volatile Box& q, int r, int& t) {    // row r of the block: its token, and its index in (T, H_q)
+      const int row = q.rb * NR + r;
       t = p.group == 1 ? row : static_cast<int>(__umulhi(static_cast<uint32_t>(row), p.group_magic));
-      return static_cast<int64_t>(q.x.q_begin + t) * p.H_q + q.head * p.group + (row - t * p.group);
+      return static_cast<int64_t>(q.q_begin + t) * p.H_q + q.head * p.group + (row - t * p.group);
     };
     // The query rows and row words of a piece are prepared by the group that owns the rows: loads first, the rest later.
-    auto load_rows = [&](const Piece& q, uint2 (&rows)[kRowsWarp]) {
+    auto load_rows = [&](const volatile Box& q, uint2 (&rows)[kRowsWarp]) {
 #pragma unroll
       for (int u = 0; u < kRowsWarp; ++u) {
         int t;
         const int64_t at = place(q, own0 + 4 * u + (warp & 3), t);
         rows[u] = make_uint2(0u, 0u);
-        if (t < q.x.q_len) rows[u] = __ldg(reinterpret_cast<const uint2*>(p.q + at * kHeadDim) + lane);
+        if (t < q.q_len) rows[u] = __ldg(reinterpret_cast<const uint2*>(p.q + at * kHeadDim) + lane);
       }
     };
-    auto prepare_rows = [&](const Piece& q, const uint2 (&rows)[kRowsWarp], int set) {
+    auto prepare_rows = [&](const volatile Box& q, uint2 (&rows)[kRowsWarp], int set) {
       if (gtid < C::kOwn) {
         int t;
         const int64_t at = place(q, own0 + gtid, t);
-        const bool real = t < q.x.q_len;
+        const bool real = t < q.q_len;
         const int r = set * NR + own0 + gtid;
-        const unsigned long long m = real && p.tree_mask ? static_cast<unsigned long long>(p.tree_mask[q.x.q_begin + t]) : 0ull;
+        const unsigned long long m = real && p.tree_mask ? static_cast<unsigned long long>(p.tree_mask[q.q_begin + t]) : 0ull;
         reinterpret_cast<unsigned long long*>(sm + C::kOffMask)[r] = m;
-        reinterpret_cast<int*>(sm + C::kOffPos)[r] = q.x.ctx + (!real ? 0 : p.tree_mask ? max(__popcll(m) - 1, 0) : t);
+        reinterpret_cast<int*>(sm + C::kOffPos)[r] = q.ctx + (!real ? 0 : p.tree_mask ? max(__popcll(m) - 1, 0) : t);
         reinterpret_cast<float*>(sm + C::kOffSlope)[r] = p.slopes && real ? p.slopes[at % p.H_q] * kLog2e : 0.f;
         float* ref = reinterpret_cast<float*>(sm + C::kOffRef) + 2 * set * NR + own0 + gtid;
         ref[0] = ref[NR] = kNoRef;
       }
-      constexpr int kBatch = kRowsWarp < 4 ? kRowsWarp : 4;
+      // two rows at a time, in a loop: what runs once a piece is kept short, or it comes out of L2 line by line each time
+#pragma unroll 1
+      for (int u = 0; u < kRowsWarp; u += kPair) {
+        float f[kPair][4];
 #pragma unroll
-      for (int u0 = 0; u0 < kRowsWarp; u0 += kBatch) {
-        float f[kBatch][4];
-#pragma unroll
-        for (int v = 0; v < kBatch; ++v) {
-          const __half2 a = *reinterpret_cast<const __half2*>(&rows[u0 + v].x), b = *reinterpret_cast<const __half2*>(&rows[u0 + v].y);
+        for (int v = 0; v < kPair; ++v) {
+          const __half2 a = *reinterpret_cast<const __half2*>(&rows[v].x), b = *reinterpret_cast<const __half2*>(&rows[v].y);
           f[v][0] = __low2float(a); f[v][1] = __high2float(a); f[v][2] = __low2float(b); f[v][3] = __high2float(b);
         }
 #pragma unroll
-        for (int v = 0; v < kBatch; ++v) fht128_warp(f[v], lane);
+        for (int v = 0; v + kPair < kRowsWarp; ++v) rows[v] = rows[v + kPair];
 #pragma unroll
-        for (int v = 0; v < kBatch; ++v) {
+        for (int v = 0; v < kPair; ++v) fht128_warp(f[v], lane);
+#pragma unroll
+        for (int v = 0; v < kPair; ++v) {
           float lo[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -507,7 +530,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
             lo[c] = f[v][c] - round_to_half(f[v][c]);
           }
           const uint2 h = pack_half4(f[v]), l = pack_half4(lo);
-          const uint32_t at = base + C::kOffQ + (lane >> 4) * (NR * 128) + sw128(own0 + 4 * (u0 + v) + (warp & 3), (lane & 15) >> 1) + 8 * (lane & 1);
+          const uint32_t at = base + C::kOffQ + (lane >> 4) * (NR * 128) + sw128(own0 + 4 * (u + v) + (warp & 3), (lane & 15) >> 1) + 8 * (lane & 1);
           sts64(at, h.x, h.y);
           sts64(at + NR * 256, l.x, l.y);
         }
@@ -518,24 +541,26 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     };
     const int my_o = C::kColO + stream * NR + col0;
     int done = 0, set = 0;                                      // tiles of the pieces so far; which set of row words
-    Piece pc, nx;
     uint2 rows[kRowsWarp];
-    bool more = w.next(p, pc);
+    if (lane == 0) { boxes[1].walk_e = w.e; boxes[1].walk_h = w.h; boxes[1].walk_j = w.j; boxes[1].walk_left = w.left; }
+    __syncwarp();
+    bool more = next_piece(1, 0);
     if (more) {
-      load_rows(pc, rows);
-      prepare_rows(pc, rows, set);
+      load_rows(boxes[0], rows);
+      prepare_rows(boxes[0], rows, set);
     }
     while (more) {
+      const volatile Box& pc = boxes[set];
       named_barrier(5, 512);                                    // the row words of both groups
-      const int ctx = pc.x.ctx, seq_len = pc.x.seq_len, end = done + pc.n;
+      const int ctx = pc.ctx, seq_len = pc.seq_len, end = done + pc.n;
       const uint32_t ref_a = base + C::kOffRef + 4 * ((2 * set + stream) * NR + col0);
       const int* pos_w = reinterpret_cast<const int*>(sm + C::kOffPos) + set * NR + col0;
       const float* slope_w = reinterpret_cast<const float*>(sm + C::kOffSlope) + set * NR + col0;
       const uint32_t* mask_w = reinterpret_cast<const uint32_t*>(sm + C::kOffMask) + 2 * (set * NR + col0);
       // tiles (by their number in all pieces) whose keys every row sees: [see_lo, see_hi)
       const int tile_at = pc.tile0 - done;                      // key tile = number + tile_at
-      const int see_hi = p.slopes ? done : (ctx + (p.tree_mask ? 0 : pc.x.t0 + 1)) / kKeys - tile_at;
-      const int see_lo = p.window > 0 ? max(0, ctx + pc.x.q_len - p.window + kKeys) / kKeys - tile_at : done;
+      const int see_hi = p.slopes ? done : (ctx + (p.tree_mask ? 0 : pc.t0 + 1)) / kKeys - tile_at;
+      const int see_lo = p.window > 0 ? max(0, ctx + pc.q_len - p.window + kKeys) / kKeys - tile_at : done;
       uint64_t sum[C::kCols / 2];
 #pragma unroll
       for (int c = 0; c < C::kCols / 2; ++c) sum[c] = f2_pack(0.f, 0.f);
@@ -556,7 +581,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
         const bool rule = i >= see_hi || i < see_lo, finish = rule || p.softcap > 0.f;
         if (finish) {                                           // cap, bias and masks, in the base-2 domain, eight columns at a time
           const int n = (i + tile_at) * kKeys + key, j = n - ctx;
-          const int pos_k = rule && p.tree_mask && j >= 0 && n < seq_len ? ctx + depth_of(p, pc.x.q_begin, j) : n;
+          const int pos_k = rule && p.tree_mask && j >= 0 && n < seq_len ? ctx + depth_of(p, pc.q_begin, j) : n;
           const int word = (j >> 5) & 1, up = 31 - (j & 31);    // bit j of a row's mask to the sign
           const uint32_t all = j < 0 ? 0x80000000u : 0u, none = n < seq_len ? 0xffffffffu : 0u;
           const float f1 = p.softcap > 0.f ? inv_cap : kf;
@@ -603,16 +628,18 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
           const int c0 = blk * C::kBlock;
           float e[C::kBlock];
 #pragma unroll 1
-          for (bool again = false;; again = true) {
+          for (bool again = first;; again = true) {              // a first tile has no references: the slow path at once
             if (blk > 0 || again) tmem_load<C::kBlock>(lanes + C::kColS + (i & (C::kSBuffers - 1)) * NR + col0 + c0, s);
             tmem_wait_ld();
             if (again) {
               // slow path: row maxima of the tile, new references, factors for what the rows hold already
+              float top = 0.f;
 #pragma unroll
               for (int c = 0; c < C::kBlock; ++c) {
                 const float m = warp_max(fmaf(__uint_as_float(s[c]), finish ? 1.0f : kf, lg));
-                if (lane == 0) sts_f(max_a + 4 * ((warp & 3) * C::kCols + c), m);
+                top = lane == c ? m : top;
               }
+              if (lane < C::kBlock) sts_f(max_a + 4 * ((warp & 3) * C::kCols + lane), top);
               group_barrier(group);
               if (gtid < C::kBlock) {
                 float m = lds_f(max_a + 4 * gtid);
@@ -642,7 +669,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
 #pragma unroll
               for (int u = 0; u < 4; ++u) a[u] = fast_exp2(a[u]);
             }
-            if (C::kStreams == 1 && blk == 0 && !again && i >= 1) {       // P and O of the last tile are at rest
+            if (C::kStreams == 1 && blk == 0 && again == first && i >= 1) {       // P and O of the last tile are at rest
               if ((warp & 3) == 0) wait_for(bar(kPvDone + ((i - 1) & 1)), ((i - 1) >> 1) & 1, wait);
               group_barrier(group);
               tc_fence_after_sync();
@@ -687,8 +714,8 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       }
 
       // ---- end of the piece.  The next piece's rows go first: its scores can then be computed while this one is written out
-      more = w.next(p, nx);
-      if (more) load_rows(nx, rows);
+      more = next_piece(set, set ^ 1);
+      if (more) load_rows(boxes[set ^ 1], rows);
       if (any_tile) {
 #pragma unroll
         for (int c0 = 0; c0 < C::kCols; c0 += C::kBlock) {
@@ -709,7 +736,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       }
       named_barrier(5, 512);
       tc_fence_after_sync();
-      if (more) prepare_rows(nx, rows, set ^ 1);
+      if (more) prepare_rows(boxes[set ^ 1], rows, set ^ 1);
       // the two streams of every own row: sums, common reference, factors
       const bool both = C::kStreams == 2 && pc.n > 1, only = C::kStreams == 2 && (done & 1) != 0;       // with a single tile one stream is empty
       float* cmb = reinterpret_cast<float*>(sm + C::kOffCmb);   // [factor 0, factor 1, sum, reference][NR]
@@ -736,11 +763,12 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
         cmb[3 * NR + r] = top;
       }
       group_barrier(group);
-      const bool alive = wait->abort == 0, whole = pc.starts && pc.ends;
-      const int64_t slot = static_cast<int64_t>(2) * blockIdx.x + (pc.starts ? 1 : 0);
+      const int edges = pc.edges;
+      const bool alive = wait->abort == 0, whole = edges == 3, starts = (edges & 2) != 0;
+      const int64_t slot = static_cast<int64_t>(2) * blockIdx.x + (starts ? 1 : 0);
       if (!whole) {
-        if (pc.starts) { rec.tail_e = pc.e; rec.tail_head = pc.head; }
-        else rec.head_state = pc.ends ? 2 : 1;
+        if (starts) { rec.tail_e = pc.e; rec.tail_head = pc.head; }
+        else rec.head_state = (edges & 1) ? 2 : 1;
         if (gtid < C::kOwn && alive)
           space.ml[slot * NR + own0 + gtid] = make_float2(cmb[3 * NR + own0 + gtid], cmb[2 * NR + own0 + gtid]);
       }
@@ -776,26 +804,31 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
 #pragma unroll
         for (int c = 0; c < C::kChunk; ++c) sts_f(area + c * 512 + key * 4, o[c]);
         group_barrier(group);
-        float v[kRowsChunk][4];
+        constexpr int kTwo = kRowsChunk < 2 ? 1 : 2;
+#pragma unroll 1
+        for (int u0 = 0; u0 < kRowsChunk; u0 += kTwo) {
+          float v[kTwo][4];
 #pragma unroll
-        for (int u = 0; u < kRowsChunk; ++u) {
-          const float l = cmb[2 * NR + ch + 4 * u + (warp & 3)], inv = l > 0.f ? kRsqrtD / l : (l == 0.f ? 0.f : l);
-          const uint4 v4 = lds128(area + (4 * u + (warp & 3)) * 512 + lane * 16);
-          v[u][0] = __uint_as_float(v4.x) * inv; v[u][1] = __uint_as_float(v4.y) * inv;
-          v[u][2] = __uint_as_float(v4.z) * inv; v[u][3] = __uint_as_float(v4.w) * inv;
-        }
+          for (int u = 0; u < kTwo; ++u) {
+            const int r = 4 * (u0 + u) + (warp & 3);
+            const float l = cmb[2 * NR + ch + r], inv = l > 0.f ? kRsqrtD / l : (l == 0.f ? 0.f : l);
+            const uint4 v4 = lds128(area + r * 512 + lane * 16);
+            v[u][0] = __uint_as_float(v4.x) * inv; v[u][1] = __uint_as_float(v4.y) * inv;
+            v[u][2] = __uint_as_float(v4.z) * inv; v[u][3] = __uint_as_float(v4.w) * inv;
+          }
 #pragma unroll
-        for (int u = 0; u < kRowsChunk; ++u) fht128_warp(v[u], lane);
+          for (int u = 0; u < kTwo; ++u) fht128_warp(v[u], lane);
 #pragma unroll
-        for (int u = 0; u < kRowsChunk; ++u) {
-          const int r = ch + 4 * u + (warp & 3);
-          int t;
-          const int64_t at = place(pc, r, t);
-          if (t < pc.x.q_len && alive) {
-            *reinterpret_cast<uint2*>(p.out + at * kHeadDim + 4 * lane) = pack_half4(v[u]);
-            if (p.lse_out && lane == 0) {
-              const float l = cmb[2 * NR + r];
-              p.lse_out[at] = l == 0.f ? -INFINITY : (log2f(l) + cmb[3 * NR + r]) * kLn2;
+          for (int u = 0; u < kTwo; ++u) {
+            const int r = ch + 4 * (u0 + u) + (warp & 3);
+            int t;
+            const int64_t at = place(pc, r, t);
+            if (t < pc.q_len && alive) {
+              *reinterpret_cast<uint2*>(p.out + at * kHeadDim + 4 * lane) = pack_half4(v[u]);
+              if (p.lse_out && lane == 0) {
+                const float l = cmb[2 * NR + r];
+                p.lse_out[at] = l == 0.f ? -INFINITY : (log2f(l) + cmb[3 * NR + r]) * kLn2;
+              }
             }
           }
         }
@@ -804,7 +837,6 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       named_barrier(5, 512);                                    // O and the P buffers may be overwritten
       tc_fence_after_sync();
       done = end;
-      pc = nx;
       set ^= 1;
     }
   } else if (warp < C::kWarpS) {
@@ -982,14 +1014,16 @@ template <int NR>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const AttendParams p, void* ws, int ctas) {
   const Space<NR> space(ws, ctas);
   const int c = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  asm volatile("griddepcontrol.wait;" ::: "memory");            // launched while the first kernel still runs
   const Record rec = space.rec[c];
+  const int state1 = c + 1 + lane < ctas ? space.rec[c + 1 + lane].head_state : 3;
   if (rec.tail_e < 0) return;
   const Entry x = entry_of<NR>(p, rec.tail_e);
   const int row = x.rb * NR + r, t = row / p.group;
   if (t >= x.q_len) return;
   int pieces = 0;                                               // CTA c's own, then those of the CTAs up to the one where it ends
   for (int k0 = c + 1; k0 < ctas; k0 += 32) {
-    const int state = k0 + lane < ctas ? space.rec[k0 + lane].head_state : 3;
+    const int state = k0 == c + 1 ? state1 : k0 + lane < ctas ? space.rec[k0 + lane].head_state : 3;
     const uint32_t stop = __ballot_sync(0xffffffffu, state != 1);
     if (stop) {
       const int at = __ffs(stop) - 1;
@@ -1005,18 +1039,16 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const AttendParams p, v
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < pieces; ++k) {
     const int64_t at = piece_row(k);
     const float2 ml = space.ml[at];
     const float4 v = reinterpret_cast<const float4*>(space.o + at * kHeadDim)[lane];
-    if (ml.x == -INFINITY) {                                    // the row saw no key in this piece (its sum is 0, or NaN)
-      l += ml.y;
-      continue;
-    }
-    const float f = exp2f(ml.x - top);
+    const bool seen = ml.x != -INFINITY;                        // else the row saw no key in this piece (its sum is 0, or NaN)
+    const float f = seen ? exp2f(ml.x - top) : 1.0f;
     l = fmaf(f, ml.y, l);
-    o[0] = fmaf(f, v.x, o[0]); o[1] = fmaf(f, v.y, o[1]); o[2] = fmaf(f, v.z, o[2]); o[3] = fmaf(f, v.w, o[3]);
+    o[0] = seen ? fmaf(f, v.x, o[0]) : o[0]; o[1] = seen ? fmaf(f, v.y, o[1]) : o[1];
+    o[2] = seen ? fmaf(f, v.z, o[2]) : o[2]; o[3] = seen ? fmaf(f, v.w, o[3]) : o[3];
   }
   const float inv = l > 0.f ? kRsqrtD / l : (l == 0.f ? 0.f : l);
 #pragma unroll
