@@ -43,7 +43,9 @@ __device__ __forceinline__ int2 remote_int2(uint32_t addr) {
 // once and kept in shared memory as ordered keys (slices too long for it are read again in every pass); the threshold is found
 // by radix selection, 11 + 11 + 10 bits, with the CTAs' histograms added up over distributed shared memory; then every warp
 // counts and writes what it keeps of its part in ascending order.  Reading the row once is the floor (256 rows of 65536: 67 MB,
-// 10 us; measured 113 us, most of it the first histogram's colliding shared-memory additions and the two ordered passes).
+// 10 us; measured 104 us: two CTAs of 16384 keys fit an SM, a CTA takes 26 us -- 3.4 for the first pass over its keys, 2.5 for each
+// of the other two, 1.7 to count, 4.1 to write, the rest in barriers, remote bins and scans -- and there are 3.5 rounds of them;
+// with 1024 threads a CTA 129 us).
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kDigitBits = 11, kBins = 1 << kDigitBits;
 constexpr int kSliceMax = 32768;                  // keys in shared memory (128 KB)
 
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    constexpr int kBatch = 8;                     // keys of a thread in flight
+    constexpr int kBatch = 16;                    // keys of a thread in flight
     for (int i0 = s0 + tid; i0 < s1; i0 += kBatch * kSelectThreads) {
       uint32_t k[kBatch];
 #pragma unroll
@@ -163,12 +165,18 @@ __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float
   // has a contiguous part of the slice.
   const int part = slice / kSelectWarps, p0 = min(s0 + warp * part, s1), p1 = min(p0 + part, s1);
   int above = 0, equal = 0;
-  for (int i0 = p0; i0 < p1; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t k = i < p1 ? key_at(i) : 0u;
-    above += __popc(__ballot_sync(0xffffffffu, i < p1 && k > prefix));
-    equal += __popc(__ballot_sync(0xffffffffu, i < p1 && k == prefix));
+  for (int i0 = p0 + lane; i0 < p1; i0 += 256) {
+    uint32_t k[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) k[u] = i0 + 32 * u < p1 ? key_at(i0 + 32 * u) : 0u;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {                 // (the key 0 is no weight's)
+      above += k[u] > prefix;
+      equal += k[u] == prefix;
+    }
   }
+  above = __reduce_add_sync(0xffffffffu, above);
+  equal = __reduce_add_sync(0xffffffffu, equal);
   if (lane == 0) s_part[warp] = make_int2(above, equal);
   __syncthreads();
   int2 before = make_int2(0, 0), all = make_int2(0, 0);
@@ -189,15 +197,21 @@ __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float
     }
   }
   int at = sink + before.x + min(before.y, left), eq_seen = before.y;      // kept and equal ones in front of this warp's part
-  for (int i0 = p0; i0 < p1; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t k = i < p1 ? key_at(i) : 0u, lower = (1u << lane) - 1u;
-    const uint32_t eq = __ballot_sync(0xffffffffu, i < p1 && k == prefix);
-    const bool take = i < p1 && (k > prefix || (k == prefix && eq_seen + __popc(eq & lower) < left));
-    const uint32_t taken = __ballot_sync(0xffffffffu, take);
-    if (take) out[at + __popc(taken & lower)] = i;
-    at += __popc(taken);
-    eq_seen += __popc(eq);
+  const uint32_t lower = (1u << lane) - 1u;
+  for (int i0 = p0; i0 < p1; i0 += 128) {         // 128 keys at a time, loads first
+    uint32_t k[4], eq[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) k[u] = i0 + 32 * u + lane < p1 ? key_at(i0 + 32 * u + lane) : 0u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) eq[u] = __ballot_sync(0xffffffffu, k[u] == prefix);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool take = k[u] > prefix || (k[u] == prefix && eq_seen + __popc(eq[u] & lower) < left);
+      const uint32_t taken = __ballot_sync(0xffffffffu, take);
+      if (take) out[at + __popc(taken & lower)] = i0 + 32 * u + lane;
+      at += __popc(taken);
+      eq_seen += __popc(eq[u]);
+    }
   }
   if (ranks > 1) cluster_sync();                  // nobody leaves while its shared memory may be read
 }

@@ -60,8 +60,10 @@ struct Cfg {
   static constexpr int kSoftWarps = 16, kProducerWarps = 12;     // four softmax groups; two K groups, one V group
   static constexpr int kWarpK = kSoftWarps, kWarpV = kWarpK + 8, kWarpS = kWarpV + 4, kWarpO = kWarpS + 1, kWarpFeed = kWarpO + 1;
   static constexpr int kThreads = (kWarpFeed + kFeeders) * 32;   // 32 warps: registers are handed out by four warps
-  // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536)
-  static constexpr int kRegsSoft = 88, kRegsK = 40, kRegsV = 40, kRegsOther = 40;
+  // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536, or 80 and
+  // 48: producers of the smaller blocks then have more look-ups in flight -- 16 trees of 64 rows 138 us, with 88 and 40 143 us;
+  // one tree of 128 rows over 131k keys 199 us with 88 and 40, 214 us with 80 and 48)
+  static constexpr int kRegsSoft = NR == 128 ? 88 : 80, kRegsOther = 128 - kRegsSoft;
   static constexpr int kRing = NR == 128 ? 2 : 4;
   static_assert(kRing % 2 == 0, "one K group reads a stage, and so sees every phase of its barrier");
   static constexpr int kTmemCols = 512;                          // tensor memory: two K, the S, one O for each stream
@@ -844,8 +846,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     // four warps for K, each with every second tile, and one for V; a thread expands one row.  The loops are kept short: unrolled
     // over the row, they evict one another (and the softmax) from the instruction caches and everything runs 1.5 times slower ==
     const bool is_v = warp >= C::kWarpV;
-    if (is_v) lower_registers<C::kRegsV>();
-    else lower_registers<C::kRegsK>();
+    lower_registers<C::kRegsOther>();
     const int step = is_v ? 1 : 2, begin = is_v ? 0 : (warp >> 2) & 1;
     const int key = (warp & 3) * 32 + lane, bits = is_v ? p.v_bits : p.k_bits;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + C::kColK;
