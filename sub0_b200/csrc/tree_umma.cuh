@@ -10,9 +10,10 @@
 // since a lane is a key, the K producers hand their expanded rows to the tensor core through tensor memory, lane by lane,
 // without a pass through shared memory.
 //
-// Warps: four softmax groups, two K producer groups and one V producer group of four warps each (a thread is a key), two MMA issuers, and two feeders that bring the slots into a ring in shared memory with tensor-map copies of
-// 16 slots of one head.  In a group that waits, one warp polls and the others are parked on a named barrier, where they take no
-// issue slots (27 polling warps spent a third of the kernel's instructions).
+// Warps: four softmax groups, two K producer groups and one V producer group of four warps each (a thread is a key), two MMA
+// issuers, and two feeders that bring the slots into a ring in shared memory with tensor-map copies of 16 slots of one head.  In
+// a group that waits, one warp polls and the others are parked on a named barrier, where they take no issue slots (27 polling
+// warps spent a third of the kernel's instructions).
 // A CTA walks an equal share of all (sequence, row block, KV head) segments' tiles; a segment that starts and ends in one CTA
 // is finished there, the pieces of the others are merged by tree_merge_kernel.
 //
@@ -36,6 +37,7 @@ constexpr int kStageBytes = kKeys * 144;         // 128 slots side by side; thei
 constexpr int kCopies = 8;                       // of the value table, one for every four lanes: 8 KB and about two wavefronts a
 constexpr int kRowShift = 5;                     // look-up (32 copies: 32 KB, one wavefront, and one ring stage less)
 constexpr uint32_t kRowMask = 255u << kRowShift; // a table row is 4 * kCopies bytes
+constexpr float kCopyStep = 1.0f / kCopies;      // copy c of the table is scaled by 2^(c * kCopyStep)
 constexpr float kNoRef = 1.0e30f;                // stored negated reference of a row without one: any score exceeds it
 constexpr float kSafe = 14.0f;
 constexpr int kFeeders = 2, kFeedIdBytes = 256;   // block ids: two chunks of four tiles for each feeder
@@ -854,9 +856,14 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     const uint32_t norm_at = 16 * (p.k_bits + p.v_bits), row0 = base + C::kOffV;
     const float* levels = reinterpret_cast<const float*>(sm + C::kOffLevels) + (is_v ? 16 : 0);
     const uint32_t tab_a = base + C::kOffTab + 4 * (lane & (kCopies - 1));
-    if (is_v && bits == 4) {                                    // the V warps fill the value table
-      for (int k = tid - C::kWarpV * 32; k < 256 * kCopies; k += 128)
-        *reinterpret_cast<uint32_t*>(sm + C::kOffTab + 4 * k) = pack_half2(levels[k / (16 * kCopies)], levels[(k / kCopies) & 15]);
+    if (is_v && bits == 4) {
+      // The V warps fill the value table.  Copy c holds the levels times 2^(c / 8), its keys' norms the inverse: a level's rounding
+      // to fp16 would else be the same for every key, a bias that stays while the outputs of a long context average out (131k keys:
+      // error against 64 bits 7.3e-4 of the output with equal copies)
+      for (int k = tid - C::kWarpV * 32; k < 256 * kCopies; k += 128) {
+        const float by = exp2f(kCopyStep * static_cast<float>(k & (kCopies - 1)));
+        *reinterpret_cast<uint32_t*>(sm + C::kOffTab + 4 * k) = pack_half2(levels[k / (16 * kCopies)] * by, levels[(k / kCopies) & 15] * by);
+      }
     }
     const int id = is_v ? 6 : 7 + begin;                        // named barriers: V 6; K 7, 8
     int stage = begin, wraps = 0;                               // of the ring
@@ -895,7 +902,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
         const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
         if (!is_v) {                                                      // (eight tiles deep: read before S of tile i + 4 is written)
           const float nv = fminf(fmaxf(__uint_as_float(norms.y), 1.0e-30f), 1.0e30f);
-          sts_f(base + C::kOffVal + 4 * ((i & 7) * kKeys + key), p.v_bits == 4 && live ? __log2f(nv) : 0.f);
+          sts_f(base + C::kOffVal + 4 * ((i & 7) * kKeys + key), p.v_bits == 4 && live ? __log2f(nv) - kCopyStep * static_cast<float>(key & (kCopies - 1)) : 0.f);
         }
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {                                     // 32 coordinates at a time
