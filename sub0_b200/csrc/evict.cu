@@ -321,11 +321,11 @@ extern "C" int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, 
                                     int64_t mass_stride, int budget, int sink, int recent, void* stream) {
   if (B < 0 || H_kv <= 0 || mass_stride < 0 || budget <= 0 || sink < 0 || recent < 0) return fail(CDA_ERR_BAD_ARG, "select_keys: negative size or no budget");
   if (static_cast<int64_t>(sink) + recent > budget) return fail(CDA_ERR_BAD_SHAPE, "select_keys: sink %d + recent %d exceed the budget %d", sink, recent, budget);
-  if (mass_stride > 0x7fffffffll || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "select_keys: too many weights or rows");
+  if (mass_stride > 0x7fff0000ll || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "select_keys: too many weights or rows");
   if (B == 0) return CDA_OK;
   if (!mass || !seq_lens || !keep || !new_lens) return fail(CDA_ERR_BAD_ARG, "select_keys: null pointer");
   // CTAs of a row: as few as hold a slice of 16384 keys each, since adding up the histograms costs a CTA as much as some 10000
-  // keys (256 rows of 65536: 113 us with 4 CTAs a row, 215 with 8, 127 with 2); more where rows are few and the GPU idle
+  // keys (256 rows of 65536: 104 us with 4 CTAs a row; before the last step 113 us with 4, 215 with 8, 127 with 2); more where rows are few and the GPU idle
   const int rows = B * H_kv, sms = device_sm_count(-1);
   int ranks = 1;
   while (ranks < 8 && (mass_stride > 16384ll * ranks || (mass_stride > 2048ll * ranks && rows * ranks <= sms / 2))) ranks *= 2;

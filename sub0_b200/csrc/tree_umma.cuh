@@ -20,6 +20,13 @@
 // The reference of a row is the largest score of the first tile in which it sees a key; it moves only when a later score is
 // more than 2^14 above it (an fp16 probability carries 2^15): then, and in a row's first tile, the group of warps takes the
 // slow path, which finds the tile's row maxima across lanes and rescales O and the sums.
+//
+// Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 133 us (slots: 20 us at copy
+// bandwidth); one tree of 32 x 4 rows over 131k keys 211 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 756 us, 364
+// TFLOP/s.  What bounds it: blocks of up to 64 rows wait for the producers -- a tile takes the V group 3700 cycles, of which 2400
+// are its look-ups, and each K group 7500 for every second tile, while the tensor cores are busy 18% of the time; blocks of 128
+// rows for the softmax (5000 of 5400 cycles a tile), whose rows are a tile's longest chain.  A new piece costs 12 to 16 us beside
+// its tiles: query rows, references, the way back, in code that has to come out of L2.
 #pragma once
 #include "attend.cuh"
 #include "cache_map.cuh"
@@ -299,13 +306,13 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int2* s_scan, 
   const int tiles_before = x - tiles + __reduce_add_sync(0xffffffffu, lane < warp ? s.x : 0);
   const int used_before = y - used + __reduce_add_sync(0xffffffffu, lane < warp ? s.y : 0);
   const int all_tiles = __reduce_add_sync(0xffffffffu, s.x), all_used = __reduce_add_sync(0xffffffffu, s.y);
-  const int64_t line = static_cast<int64_t>(all_tiles + kPieceCost<NR> * all_used) * p.H_kv;
+  const int64_t line = (all_tiles + static_cast<int64_t>(kPieceCost<NR>) * all_used) * p.H_kv;
   const int busy = static_cast<int>(line < gridDim.x ? line : gridDim.x), cta = min(static_cast<int>(blockIdx.x), busy);
   const int64_t lo = busy ? line * cta / busy : 0, hi = cta < busy ? line * (cta + 1) / busy : lo;
   if (tid == 0) s_plan[3] = *s_end = 0;
   __syncthreads();
-  int64_t at = static_cast<int64_t>(tiles_before + kPieceCost<NR> * used_before) * p.H_kv;
-  const int64_t mine = static_cast<int64_t>(tiles + kPieceCost<NR> * used) * p.H_kv;
+  int64_t at = (tiles_before + static_cast<int64_t>(kPieceCost<NR>) * used_before) * p.H_kv;
+  const int64_t mine = (tiles + static_cast<int64_t>(kPieceCost<NR>) * used) * p.H_kv;
   if (hi > lo && hi > at && lo < at + mine) {                    // the line's positions lo or hi - 1 may lie in these entries
     int real = tiles_before * p.H_kv;
     for (int e = e0; e < e1; ++e) {
@@ -345,7 +352,8 @@ __device__ __forceinline__ void copy_group(uint32_t dst, const CUtensorMap* map,
 // Tiles [tile0, tile0 + n) of a piece, as the feeders see it.
 struct Feed { int b, head, seq_len, tile0, n; };
 // A feeder warp: copies every kFeeders-th tile of the CTA's walk to the ring, one lane per 16-token group.  A lane's copy takes
-// about 90 cycles to issue, eight of them and the stage's bookkeeping 1250: two warps, or the ring is never full.  Block ids
+// about 90 cycles to issue, eight of them and the stage's bookkeeping 1250: two warps, or the ring is never full
+// (4 trees of 512 rows: 734 us with one, 703 with two).  Block ids
 // come four tiles at a time (one a lane), asynchronously into shared memory while the chunk before them is copied -- a load into a
 // register was waited for at once, 2000 cycles under load -- across the end of a piece too.  Each feeder sees every phase of its
 // stages' barriers.

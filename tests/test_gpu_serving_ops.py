@@ -417,6 +417,37 @@ def test_many_tiles_per_cta(B, N, group, k_bits, v_bits):
     assert ops.kv_status() == 0
 
 
+def check_mass(c, lse):
+    from sub0_b200 import ops
+    start = torch.zeros(len(c["q_lens"]), c["H_kv"], int(c["seq_lens"].max()))
+    mass = on(start).clone()
+    ops.attention_mass(on(c["Q"]), on(c["cache"]), on(c["block_table"]), on(c["seq_lens"]), on(lse), mass, **call_args(c))
+    assert ops.kv_status() == 0
+    want, tol = S.mass_reference(c, lse, start)
+    off = float(((mass.double().cpu() - want).abs() / tol).max())
+    assert off <= 1.0, f"mass is {off:.2f} bounds off"
+
+
+@pytest.mark.parametrize("H_kv", [1, 3, 6, 7, 11, 12, 16, 33])
+def test_numbers_of_heads(H_kv):
+    """Neighbouring CTAs walk the heads of a token together, in teams of the largest divisor up to eight."""
+    c = S.attend_case([300, 5, 0, 900, 129], [3, 5, 0, 2, 1], H_kv=H_kv, group=2, seed=H_kv)
+    check_tree(c, *run_tree(c))
+    check_mass(c, S.tree_reference(c)[2].float())
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5, 16])
+def test_many_pieces_per_cta(rows):
+    """Hundreds of short sequences, some empty: a CTA starts and ends dozens of pieces, most of a single tile."""
+    gen = torch.Generator().manual_seed(rows)
+    lens = [int(v) for v in torch.randint(0, 300, (700,), generator=gen)]
+    lens[::5] = [v % 7 for v in lens[::5]]
+    q_lens = [min(v, 1 + int(r)) for v, r in zip(lens, torch.randint(0, rows, (700,), generator=gen))]
+    c = S.attend_case(lens, q_lens, H_kv=4, group=4, seed=rows)
+    check_tree(c, *run_tree(c))
+    check_mass(c, S.tree_reference(c)[2].float())
+
+
 def test_refusals_on_the_gpu():
     """Arguments that the front end refuses before anything is launched."""
     from sub0_b200 import ops
