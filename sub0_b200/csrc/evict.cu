@@ -43,7 +43,7 @@ __device__ __forceinline__ int2 remote_int2(uint32_t addr) {
 // once and kept in shared memory as ordered keys (slices too long for it are read again in every pass); the threshold is found
 // by radix selection, 11 + 11 + 10 bits, with the CTAs' histograms added up over distributed shared memory; then every warp
 // counts and writes what it keeps of its part in ascending order.  Reading the row once is the floor (256 rows of 65536: 67 MB,
-// 10 us; measured 104 us: two CTAs of 16384 keys fit an SM, a CTA takes 26 us -- 3.4 for the first pass over its keys, 2.5 for each
+// 10 us; measured 101 us: two CTAs of 16384 keys fit an SM, a CTA takes 26 us -- 3.4 for the first pass over its keys, 2.5 for each
 // of the other two, 1.7 to count, 4.1 to write, the rest in barriers, remote bins and scans -- and there are 3.5 rounds of them;
 // with 1024 threads a CTA 129 us).
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kDigitBits = 11, kBins = 1 << kDigitBits;
@@ -206,11 +206,14 @@ __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float
     for (int u = 0; u < 4; ++u) eq[u] = __ballot_sync(0xffffffffu, k[u] == prefix);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const bool take = k[u] > prefix || (k[u] == prefix && eq_seen + __popc(eq[u] & lower) < left);
+      bool take = k[u] > prefix;
+      if (eq[u]) {                                // some at the threshold: the first `left` of the row
+        take = take || (k[u] == prefix && eq_seen + __popc(eq[u] & lower) < left);
+        eq_seen += __popc(eq[u]);
+      }
       const uint32_t taken = __ballot_sync(0xffffffffu, take);
       if (take) out[at + __popc(taken & lower)] = i0 + 32 * u + lane;
       at += __popc(taken);
-      eq_seen += __popc(eq[u]);
     }
   }
   if (ranks > 1) cluster_sync();                  // nobody leaves while its shared memory may be read
@@ -221,6 +224,9 @@ __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float
 // destination, so that slots may be moved in place a step at a time: what a step reads lies at or behind the first place
 // it writes, i.e. behind everything that earlier steps wrote.  A cluster of CTAs shares a step: all read, all wait for one
 // another, all write.  A slot is 5 to 9 pieces of 16 bytes, read and written by neighbouring threads.
+// Floor: every moved slot read and written once (128 lists of 4096 of 16k slots: 23 us at copy bandwidth; measured 47 us;
+// single cold launches: 52 us with four CTAs an SM, 58 with the two that 122 registers a thread allow, 63 when a step's entries
+// are looked up while the slots of the one before are read).
 constexpr int kCompactThreads = 256, kCompactStep = 256;      // entries of one CTA in a step
 
 struct CompactParams {
@@ -236,7 +242,7 @@ struct CompactParams {
 };
 
 template <int PIECES>
-__global__ void __launch_bounds__(kCompactThreads) compact_cache_kernel(const CompactParams p) {
+__global__ void __launch_bounds__(kCompactThreads, 4) compact_cache_kernel(const CompactParams p) {
   __shared__ int64_t s_from[kCompactStep], s_to[kCompactStep];  // byte offsets of the slots, -1: nothing to move
   const int tid = threadIdx.x;
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
@@ -325,7 +331,7 @@ extern "C" int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, 
   if (B == 0) return CDA_OK;
   if (!mass || !seq_lens || !keep || !new_lens) return fail(CDA_ERR_BAD_ARG, "select_keys: null pointer");
   // CTAs of a row: as few as hold a slice of 16384 keys each, since adding up the histograms costs a CTA as much as some 10000
-  // keys (256 rows of 65536: 104 us with 4 CTAs a row; before the last step 113 us with 4, 215 with 8, 127 with 2); more where rows are few and the GPU idle
+  // keys (256 rows of 65536: 101 us with 4 CTAs a row; before the last steps 113 us with 4, 215 with 8, 127 with 2); more where rows are few and the GPU idle
   const int rows = B * H_kv, sms = device_sm_count(-1);
   int ranks = 1;
   while (ranks < 8 && (mass_stride > 16384ll * ranks || (mass_stride > 2048ll * ranks && rows * ranks <= sms / 2))) ranks *= 2;
@@ -356,7 +362,7 @@ extern "C" int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table
   if (!aligned16(kv_cache)) return fail(CDA_ERR_BAD_ALIGN, "compact_cache: cache must be 16-byte aligned");
   const CompactParams p{static_cast<uint8_t*>(kv_cache), block_table, seq_lens, keep, start, mass, mass_stride, B, H_kv, K, block_size,
                         block_table_stride, static_cast<int>(num_slots / block_size), slot_bytes, keep_heads == 1 ? 1 : 0};
-  // CTAs of a list: until each has one step, or all SMs have two (128 lists of 4096: 57 us with 4 CTAs each, 63 with 8)
+  // CTAs of a list: until each has one step, or all SMs have two (128 lists of 4096, two CTAs an SM: 57 us with 4 CTAs each, 63 with 8)
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rows = B * H_kv, sms = device_sm_count(-1);
   int ranks = 1;
