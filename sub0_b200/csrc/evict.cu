@@ -46,7 +46,7 @@ __device__ __forceinline__ int2 remote_int2(uint32_t addr) {
 // 10 us; measured 101 us: two CTAs of 16384 keys fit an SM, a CTA takes 26 us -- 3.4 for the first pass over its keys, 2.5 for each
 // of the other two, 1.7 to count, 4.1 to write, the rest in barriers, remote bins and scans -- and there are 3.5 rounds of them;
 // with 1024 threads a CTA 129 us).
-constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kDigitBits = 11, kBins = 1 << kDigitBits;
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32, kBins = 1 << 11;
 constexpr int kSliceMax = 32768;                  // keys in shared memory (128 KB)
 
 // Larger weights have larger keys; -0 counts as 0 and NaN as minus infinity, like any value below every other.

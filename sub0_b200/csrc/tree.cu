@@ -36,6 +36,8 @@ static int fill_params(AttendParams& p, const char* what, const void* Q, const v
   if (static_cast<int64_t>(bt_stride) * block_size < max_n) return fail(CDA_ERR_BAD_SHAPE, "%s: block table row shorter than max_seq_len", what);
   if (tree_mask && max_q > 64) return fail(CDA_ERR_UNSUPPORTED, "%s: a tree has at most 64 tokens, max_query_len is %d", what, max_q);
   if (num_slots > 0x7fffffffll) return fail(CDA_ERR_N_TOO_LARGE, "%s: too many slots", what);
+  // (a row's token is found by a product with 2^32 / group, exact below 2^26 rows)
+  if (static_cast<int64_t>(max_q) * (H_q / H_kv) > 1ll << 26) return fail(CDA_ERR_N_TOO_LARGE, "%s: %d new tokens of %d query heads a KV head are too many", what, max_q, H_q / H_kv);
   if (B == 0 || T == 0 || max_q == 0 || max_n == 0) return 1;
   if (num_slots < block_size) return fail(CDA_ERR_BAD_SHAPE, "%s: the cache holds no block", what);
   if (!Q || !kv_cache || !block_table || !cu_q || !seq_lens || !cb_K) return fail(CDA_ERR_BAD_ARG, "%s: null pointer", what);

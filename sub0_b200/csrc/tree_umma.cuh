@@ -66,7 +66,7 @@ struct Cfg {
   static constexpr int kBlock = kCols < 16 ? kCols : 16;         // columns worked on at a time
   static constexpr int kOwn = NR / 4;                            // rows that a group prepares and writes out,
   static constexpr int kChunk = kOwn < 16 ? kOwn : 16;           // so many at a time
-  static constexpr int kSoftWarps = 16, kProducerWarps = 12;     // four softmax groups; two K groups, one V group
+  static constexpr int kSoftWarps = 16;                          // four softmax groups; two K groups and one V group follow
   static constexpr int kWarpK = kSoftWarps, kWarpV = kWarpK + 8, kWarpS = kWarpV + 4, kWarpO = kWarpS + 1, kWarpFeed = kWarpO + 1;
   static constexpr int kThreads = (kWarpFeed + kFeeders) * 32;   // 32 warps: registers are handed out by four warps
   // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536, or 80 and

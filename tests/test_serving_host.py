@@ -43,6 +43,13 @@ def test_attention_refusals(lib, al, what, code):
     assert L.cda_b200_attention_mass(al, al, al, al, al, al, None, None, al, None, al, 100, *attend(**what)) == want
 
 
+def test_chunks_of_too_many_rows_are_refused(lib, al):
+    L = lib.lib
+    for max_q, want in (((1 << 24) + 1, lib.CDA_ERR_N_TOO_LARGE), ((1 << 24), lib.CDA_ERR_WORKSPACE)):
+        assert L.cda_b200_tree_attention(al, al, al, al, al, al, al, None, None, al, None, al, 0, *attend(max_q=max_q)) == want
+    assert L.cda_b200_attention_mass(al, al, al, al, al, al, None, None, al, None, al, 100, *attend(max_q=(1 << 24) + 1)) == lib.CDA_ERR_N_TOO_LARGE
+
+
 def test_attention_refusals_of_pointers_and_workspace(lib, al):
     L = lib.lib
     need = L.cda_b200_tree_attention_workspace_bytes(8, 2, 3, -1)
