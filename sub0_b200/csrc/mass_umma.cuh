@@ -164,8 +164,6 @@ __global__ void __launch_bounds__(MassCfg<NR>::kThreads, 1) attention_mass_kerne
   const uint32_t bar0 = base + C::kOffBar;
   auto bar = [&](int i) { return bar0 + 8u * i; };
 
-  find_mass_share<NR, C::kThreads>(p, reinterpret_cast<longlong2*>(sm + C::kOffScan), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kMOffEnd));
-  if (s_plan[3] == 0) return;
   if (tid == 0) {
     for (int i = 0; i < C::kKGroups; ++i) { mbar_init(bar(kMKFull + i), 4); mbar_init(bar(kMKEmpty + i), 1); }
     for (int i = 0; i < C::kSBuffers; ++i) { mbar_init(bar(kMSFull + i), 1); mbar_init(bar(kMSEmpty + i), 4); }
@@ -182,9 +180,13 @@ __global__ void __launch_bounds__(MassCfg<NR>::kThreads, 1) attention_mass_kerne
     tmem_relinquish();
   }
   tc_fence_before_sync();
-  __syncthreads();
+  find_mass_share<NR, C::kThreads>(p, reinterpret_cast<longlong2*>(sm + C::kOffScan), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kMOffEnd));
   tc_fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + C::kOffBar + kMOffTmem);
+  if (s_plan[3] == 0) {
+    if (warp == C::kWarpS) tmem_dealloc(tmem, C::kTmemCols);
+    return;
+  }
   MassWalk<NR> w;
   w.b = s_plan[0]; w.h = s_plan[1] * p.side + blockIdx.x % p.side; w.j = s_plan[2]; w.left = s_plan[3]; w.B = p.B; w.piece_n = 0; w.rb = 0; w.s.blocks = 0;
   Sub q;

@@ -21,7 +21,7 @@
 // more than 2^14 above it (an fp16 probability carries 2^15): then, and in a row's first tile, the group of warps takes the
 // slow path, which finds the tile's row maxima across lanes and rescales O and the sums.
 //
-// Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 133 us (slots: 20 us at copy
+// Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 129 us (slots: 20 us at copy
 // bandwidth); one tree of 32 x 4 rows over 131k keys 211 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 756 us, 364
 // TFLOP/s.  What bounds it: blocks of up to 64 rows wait for the producers -- a tile takes the V group 3700 cycles, of which 2400
 // are its look-ups, and each K group 7500 for every second tile, while the tensor cores are busy 18% of the time; blocks of 128
@@ -308,7 +308,8 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int2* s_scan, 
   const int all_tiles = __reduce_add_sync(0xffffffffu, s.x), all_used = __reduce_add_sync(0xffffffffu, s.y);
   const int64_t line = (all_tiles + static_cast<int64_t>(kPieceCost<NR>) * all_used) * p.H_kv;
   const int busy = static_cast<int>(line < gridDim.x ? line : gridDim.x), cta = min(static_cast<int>(blockIdx.x), busy);
-  const int64_t lo = busy ? line * cta / busy : 0, hi = cta < busy ? line * (cta + 1) / busy : lo;
+  const int64_t each = busy ? line / busy : 0, over = line - each * busy;           // the first `over` CTAs take one more
+  const int64_t lo = each * cta + min(static_cast<int64_t>(cta), over), hi = cta < busy ? lo + each + (cta < over ? 1 : 0) : lo;
   if (tid == 0) s_plan[3] = *s_end = 0;
   __syncthreads();
   int64_t at = (tiles_before + static_cast<int64_t>(kPieceCost<NR>) * used_before) * p.H_kv;
@@ -430,13 +431,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
   const uint32_t bar0 = base + C::kOffBar;
   auto bar = [&](int i) { return bar0 + 8u * i; };
 
-  find_share<NR, C::kThreads>(p, reinterpret_cast<int2*>(sm + C::kOffTab), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kOffPlanEnd));
-  const int total = s_plan[3];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may take its places; it waits for this kernel's end
-  if (total == 0) {
-    if (tid == 0) space.rec[blockIdx.x] = Record{-1, 0, 0, 0};
-    return;
-  }
+  // (the lengths' way from memory is long: what does not need them goes first)
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {                               // counts: warps that arrive, or one commit
       mbar_init(bar(kKFull + i), 4); mbar_init(bar(kKEmpty + i), 1); mbar_init(bar(kVFull + i), 4);
@@ -459,9 +454,16 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     tmem_relinquish();
   }
   tc_fence_before_sync();
-  __syncthreads();
+  find_share<NR, C::kThreads>(p, reinterpret_cast<int2*>(sm + C::kOffTab), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kOffPlanEnd));
   tc_fence_after_sync();
+  const int total = s_plan[3];
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + C::kOffBar + kOffTmemAddr);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may take its places; it waits for this kernel's end
+  if (total == 0) {
+    if (tid == 0) space.rec[blockIdx.x] = Record{-1, 0, 0, 0};
+    if (warp == C::kWarpS) tmem_dealloc(tmem, C::kTmemCols);
+    return;
+  }
   Walk<NR> w{s_plan[0], s_plan[1], s_plan[2], total, p.B * p.row_blocks};
   Record rec{-1, 0, 0, 0};
 
