@@ -448,6 +448,43 @@ def test_many_pieces_per_cta(rows):
     check_mass(c, S.tree_reference(c)[2].float())
 
 
+def test_two_streams_at_once():
+    """Calls of different sizes interleaved on two streams, each several times: bit for bit what the calls give alone."""
+    from sub0_b200 import ops
+    cases = [S.attend_case([700, 5000, 33], [7, 16, 1], seed=1), S.attend_case([9000, 300], [40, 3], group=8, v_bits=2, seed=2)]
+    calls = []
+    for c in cases:
+        a = call_args(c)
+        tensors = [on(c[k]) for k in ("Q", "cache", "block_table", "seq_lens", "cb_V")]
+        calls.append((a, tensors, torch.empty_like(tensors[0]), torch.empty(tensors[0].shape[:2], device=DEV),
+                      torch.zeros(len(c["q_lens"]), c["H_kv"], a["max_seq_len"], device=DEV)))
+
+    def run(a, tensors, out, lse, mass):
+        Q, cache, table, lens, cb_V = tensors
+        ops.tree_attention(Q, cache, table, lens, out, cb_V=cb_V, lse=lse, **a)
+        mass.zero_()
+        ops.attention_mass(Q, cache, table, lens, lse, mass, **a)
+
+    alone = []
+    for call in calls:
+        run(*call)
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in call[2:]])
+        for t in call[2:]:
+            t.fill_(3.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for stream, call in zip(streams, calls):
+            with torch.cuda.stream(stream):
+                run(*call)
+    torch.cuda.synchronize()
+    assert ops.kv_status() == 0
+    for call, want in zip(calls, alone):
+        for got, w in zip(call[2:], want):
+            assert torch.equal(got, w)
+
+
 def test_refusals_on_the_gpu():
     """Arguments that the front end refuses before anything is launched."""
     from sub0_b200 import ops
