@@ -448,6 +448,23 @@ def test_many_pieces_per_cta(rows):
     check_mass(c, S.tree_reference(c)[2].float())
 
 
+@pytest.mark.parametrize("max_q,more", [(17, 0), (40, 1000), (64, 500000)])
+def test_limits_above_the_lengths(max_q, more):
+    """Callers give bounds, not lengths: the call may then use larger row blocks and has idle ones."""
+    from sub0_b200 import ops
+    c = S.attend_case([700, 0, 33, 1290], [7, 0, 1, 16], seed=9)
+    wide = (int(c["seq_lens"].max()) + more + 15) // 16
+    c["block_table"] = torch.cat([c["block_table"], torch.full((4, max(0, wide - c["block_table"].shape[1])), -1, dtype=torch.int32)], 1)
+    a = dict(max_query_len=max_q, max_seq_len=int(c["seq_lens"].max()) + more)
+    out, lse = run_tree(c, **a)
+    check_tree(c, out, lse)
+    z = S.tree_reference(c)[2].float()
+    mass = torch.zeros(4, c["H_kv"], a["max_seq_len"], device=DEV)
+    ops.attention_mass(on(c["Q"]), on(c["cache"]), on(c["block_table"]), on(c["seq_lens"]), on(z), mass, **{**call_args(c), **a})
+    want, tol = S.mass_reference(c, z, torch.zeros(mass.shape))
+    assert bool(((mass.double().cpu() - want).abs() <= tol).all()) and ops.kv_status() == 0
+
+
 def test_two_streams_at_once():
     """Calls of different sizes interleaved on two streams, each several times: bit for bit what the calls give alone."""
     from sub0_b200 import ops
