@@ -76,6 +76,9 @@ static int launch_tree(AttendParams& p, void* ws, int ctas, const CUtensorMap& m
   if (dev < 0 || dev >= 64 || !configured[dev]) {
     if (cudaFuncSetAttribute(tru::tree_attention_kernel<NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, tru::Cfg<NR>::kSmemBytes) != cudaSuccess)
       return check_launch("tree_attention: shared memory opt-in");
+    cudaFuncAttributes attr;                                    // the warps share out the launch's registers; more would be waited for in vain
+    if (cudaFuncGetAttributes(&attr, tru::tree_attention_kernel<NR>) != cudaSuccess) return check_launch("tree_attention: attributes");
+    if (attr.numRegs * tru::Cfg<NR>::kThreads < tru::Cfg<NR>::kRegsAll) return fail(CDA_ERR_UNSUPPORTED, "tree_attention: built with %d registers a thread, too few", attr.numRegs);
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   tru::tree_attention_kernel<NR><<<ctas, tru::Cfg<NR>::kThreads, tru::Cfg<NR>::kSmemBytes, st>>>(p, ws, map);

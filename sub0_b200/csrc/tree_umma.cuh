@@ -67,12 +67,13 @@ struct Cfg {
   static constexpr int kOwn = NR / 4;                            // rows that a group prepares and writes out,
   static constexpr int kChunk = kOwn < 16 ? kOwn : 16;           // so many at a time
   static constexpr int kSoftWarps = 16;                          // four softmax groups; two K groups and one V group follow
-  static constexpr int kWarpK = kSoftWarps, kWarpV = kWarpK + 8, kWarpS = kWarpV + 4, kWarpO = kWarpS + 1, kWarpFeed = kWarpO + 1;
+  static constexpr int kKGroups = NR == 128 ? 1 : 2, kWarpK = kSoftWarps, kWarpV = kWarpK + 4 * kKGroups, kWarpS = kWarpV + 4, kWarpO = kWarpS + 1, kWarpFeed = kWarpO + 1;
   static constexpr int kThreads = (kWarpFeed + kFeeders) * 32;   // 32 warps: registers are handed out by four warps
   // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536, or 80 and
   // 48: producers of the smaller blocks then have more look-ups in flight -- 16 trees of 64 rows 138 us, with 88 and 40 143 us;
   // one tree of 128 rows over 131k keys 199 us with 88 and 40, 214 us with 80 and 48)
-  static constexpr int kRegsSoft = NR == 128 ? 88 : 80, kRegsOther = 128 - kRegsSoft;
+  static constexpr int kRegsSoft = NR == 128 ? 88 : 80, kRegsOther = 48;
+  static constexpr int kRegsAll = 32 * (kSoftWarps * kRegsSoft + (kThreads / 32 - kSoftWarps) * kRegsOther);   // may not exceed the launch's
   static constexpr int kRing = NR == 128 ? 2 : 4;
   static_assert(kRing % 2 == 0, "one K group reads a stage, and so sees every phase of its barrier");
   static constexpr int kTmemCols = 512;                          // tensor memory: two K, the S, one O for each stream
@@ -301,8 +302,7 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int2* s_scan, 
   }
   if (lane == 31) s_scan[warp] = make_int2(x, y);
   __syncthreads();
-  static_assert(THREADS == 1024, "a lane for every warp's total");
-  const int2 s = s_scan[lane];
+  const int2 s = lane < THREADS / 32 ? s_scan[lane] : make_int2(0, 0);   // a lane for every warp's total
   const int tiles_before = x - tiles + __reduce_add_sync(0xffffffffu, lane < warp ? s.x : 0);
   const int used_before = y - used + __reduce_add_sync(0xffffffffu, lane < warp ? s.y : 0);
   const int all_tiles = __reduce_add_sync(0xffffffffu, s.x), all_used = __reduce_add_sync(0xffffffffu, s.y);
@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     // over the row, they evict one another (and the softmax) from the instruction caches and everything runs 1.5 times slower ==
     const bool is_v = warp >= C::kWarpV;
     lower_registers<C::kRegsOther>();
-    const int step = is_v ? 1 : 2, begin = is_v ? 0 : (warp >> 2) & 1;
+    const int step = is_v ? 1 : C::kKGroups, begin = is_v || C::kKGroups == 1 ? 0 : (warp >> 2) & 1;
     const int key = (warp & 3) * 32 + lane, bits = is_v ? p.v_bits : p.k_bits;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + C::kColK;
     const uint32_t cell0 = base + C::kOffRing + key * p.slot_bytes, code_at = is_v ? 16 * p.k_bits : 0;
