@@ -60,7 +60,7 @@ using namespace cda;
 
 namespace cda {
 // Rows of a block: the smallest of 16, 32, 64, 128 that holds all rows of the longest chunk, else 128.  A block expands every tile
-// of keys once, so fewer, larger blocks win as soon as their columns are filled (512 rows a sequence: 756 us in blocks of 128,
+// of keys once, so fewer, larger blocks win as soon as their columns are filled (512 rows a sequence: 705 us in blocks of 128,
 // 966 us in blocks of 64).
 static int rows_per_block(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 

@@ -10,7 +10,7 @@
 // since a lane is a key, the K producers hand their expanded rows to the tensor core through tensor memory, lane by lane,
 // without a pass through shared memory.
 //
-// Warps: four softmax groups, two K producer groups and one V producer group of four warps each (a thread is a key), two MMA
+// Warps: four softmax groups, two K producer groups (one for 128 rows) and a V producer group of four warps each (a thread is a key), two MMA
 // issuers, and two feeders that bring the slots into a ring in shared memory with tensor-map copies of 16 slots of one head.  In
 // a group that waits, one warp polls and the others are parked on a named barrier, where they take no issue slots (27 polling
 // warps spent a third of the kernel's instructions).
@@ -22,10 +22,10 @@
 // slow path, which finds the tile's row maxima across lanes and rescales O and the sums.
 //
 // Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 129 us (slots: 20 us at copy
-// bandwidth); one tree of 32 x 4 rows over 131k keys 211 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 756 us, 364
+// bandwidth); one tree of 32 x 4 rows over 131k keys 209 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 705 us, 390
 // TFLOP/s.  What bounds it: blocks of up to 64 rows wait for the producers -- a tile takes the V group 3700 cycles, of which 2400
 // are its look-ups, and each K group 7500 for every second tile, while the tensor cores are busy 18% of the time; blocks of 128
-// rows for the softmax (5000 of 5400 cycles a tile), whose rows are a tile's longest chain.  A new piece costs 12 to 16 us beside
+// rows for the softmax (a chain of some 4500 cycles a tile) and for the clock that the power limit leaves.  A new piece costs 12 to 16 us beside
 // its tiles: query rows, references, the way back, in code that has to come out of L2.
 #pragma once
 #include "attend.cuh"
@@ -68,10 +68,11 @@ struct Cfg {
   static constexpr int kChunk = kOwn < 16 ? kOwn : 16;           // so many at a time
   static constexpr int kSoftWarps = 16;                          // four softmax groups; two K groups and one V group follow
   static constexpr int kKGroups = NR == 128 ? 1 : 2, kWarpK = kSoftWarps, kWarpV = kWarpK + 4 * kKGroups, kWarpS = kWarpV + 4, kWarpO = kWarpS + 1, kWarpFeed = kWarpO + 1;
-  static constexpr int kThreads = (kWarpFeed + kFeeders) * 32;   // 32 warps: registers are handed out by four warps
-  // registers a thread: 32 warps start with 64; softmax takes what the others give back (512 x 88 + 512 x 40 = 65536, or 80 and
-  // 48: producers of the smaller blocks then have more look-ups in flight -- 16 trees of 64 rows 138 us, with 88 and 40 143 us;
-  // one tree of 128 rows over 131k keys 199 us with 88 and 40, 214 us with 80 and 48)
+  static constexpr int kThreads = (kWarpFeed + kFeeders) * 32;   // 32 or 28 warps: registers are handed out by four
+  // Registers a thread: softmax takes what the others give back.  32 warps start with 64 (16 x 80 + 16 x 48 a lane; with 88 and 40
+  // producers have fewer look-ups in flight: 16 trees of 64 rows 143 us against 138); blocks of 128 rows, whose softmax has the
+  // longest chain, do with one K group: 28 warps start with 72 (4 trees of 512 rows 705 us; with two K groups, 88 and 40, 763 us;
+  // with 80 and 56 757 us, with 96 and 40 841 us)
   static constexpr int kRegsSoft = NR == 128 ? 88 : 80, kRegsOther = 48;
   static constexpr int kRegsAll = 32 * (kSoftWarps * kRegsSoft + (kThreads / 32 - kSoftWarps) * kRegsOther);   // may not exceed the launch's
   static constexpr int kRing = NR == 128 ? 2 : 4;
