@@ -289,7 +289,8 @@ int cda_b200_prefill_debug(int wait_limit_us, int withhold_first_k_arrive);
  *   seen  : n < ctx, or n = ctx + j with bit j of tree_mask[t] set (no mask: j <= t); and pos_t - pos_n < window if window > 0
  *   out   = sum_n softmax(x)_n v_n over the keys seen, lse = log sum_n exp(x_n); a row that sees none: zeros, -inf
  * The position of a context key is its place, that of a new token ctx + depth, its depth being its place in a chain and
- * popcount(mask) - 1 (not below 0) in a tree.
+ * popcount(mask) - 1 (not below 0) in a tree.  Mask bits at and above q_len name no token: they show no key, but count for the
+ * depth.
  *   Q, out (T, H_q, 128) fp16, 16-byte aligned; the group H_q / H_kv is at most 64     cu_seqlens_q (B+1)     seq_lens (B)
  *   tree_mask (T) int64 or null; with a mask max_query_len is at most 64               alibi_slopes (H_q) fp32 or null
  *   lse (T, H_q) fp32 or null          workspace >= cda_b200_tree_attention_workspace_bytes(...) bytes, 16-byte aligned,

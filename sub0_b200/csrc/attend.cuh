@@ -52,6 +52,10 @@ __device__ __forceinline__ int depth_of(const AttendParams& p, int q_begin, int 
   return p.tree_mask ? max(__popcll(static_cast<unsigned long long>(p.tree_mask[q_begin + t])) - 1, 0) : t;
 }
 
+// How many positions, from the context's end on, new tokens may stand at: a mask's bits at and above q_len name no token, but
+// they count for the depth (63 at most).
+__device__ __forceinline__ int positions_of(const AttendParams& p, int q_len) { return p.tree_mask ? 64 : q_len; }
+
 // tanh for capped scores.  tanh.approx is off by up to 2^-11, which on a score near a cap of 50 is 0.02 and on its
 // probability 2 %, so: below 0.55 the odd Taylor series to x^15 (truncation below 5e-8 of the value), above it 1 - 2 / (e^2x +
 // 1), where the two approximate instructions leave less than 2^-22.

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(MassCfg<NR>::kThreads, 1) attention_mass_kerne
       named_barrier(5, 256);
       const int ctx = q.s.ctx, seq_len = q.s.v.seq_len, end = done + q.n, tile_at = q.tile0 - done;
       const int see_hi = p.slopes ? done : (ctx + (p.tree_mask ? 0 : q.t0 + 1)) / kKeys - tile_at;
-      const int see_lo = p.window > 0 ? max(0, ctx + q.s.v.q_len - p.window + kKeys) / kKeys - tile_at : done;
+      const int see_lo = p.window > 0 ? max(0, ctx + positions_of(p, q.s.v.q_len) - p.window + kKeys) / kKeys - tile_at : done;
       const int cols = (rows + C::kChunk - 1) / C::kChunk * C::kChunk;
       float* mass = p.mass + (static_cast<int64_t>(q.b) * p.H_kv + q.head) * p.mass_stride;
 #pragma unroll 1

@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       // tiles (by their number in all pieces) whose keys every row sees: [see_lo, see_hi)
       const int tile_at = pc.tile0 - done;                      // key tile = number + tile_at
       const int see_hi = p.slopes ? done : (ctx + (p.tree_mask ? 0 : pc.t0 + 1)) / kKeys - tile_at;
-      const int see_lo = p.window > 0 ? max(0, ctx + pc.q_len - p.window + kKeys) / kKeys - tile_at : done;
+      const int see_lo = p.window > 0 ? max(0, ctx + positions_of(p, pc.q_len) - p.window + kKeys) / kKeys - tile_at : done;
       uint64_t sum[C::kCols / 2];
 #pragma unroll
       for (int c = 0; c < C::kCols / 2; ++c) sum[c] = f2_pack(0.f, 0.f);
