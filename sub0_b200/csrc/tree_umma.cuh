@@ -17,9 +17,11 @@
 // A CTA walks an equal share of all (sequence, row block, KV head) segments' tiles; a segment that starts and ends in one CTA
 // is finished there, the pieces of the others are merged by tree_merge_kernel.
 //
-// The reference of a row is the largest score of the first tile in which it sees a key; it moves only when a later score is
-// more than 2^14 above it (an fp16 probability carries 2^15): then, and in a row's first tile, the group of warps takes the
-// slow path, which finds the tile's row maxima across lanes and rescales O and the sums.
+// The reference of a row lies 2^10 below the largest score of the first tile in which it sees a key; it moves only when a later
+// score is more than 2^15.5 above it (an fp16 probability ends at 2^16): then, and in a row's first tile, the group of warps
+// takes the slow path, which finds the tile's row maxima across lanes and rescales O and the sums.  The distance keeps keys
+// down to 2^-24 of the largest (17 nats below it) in fp16's normal range: where one key draws nearly all attention and has a
+// small value row, they are the output.  (With the reference at the maximum, such an output of 1500 keys was off by 2 %.)
 //
 // Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 129 us (slots: 20 us at copy
 // bandwidth); one tree of 32 x 4 rows over 131k keys 209 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 705 us, 390
@@ -46,7 +48,7 @@ constexpr int kRowShift = 5;                     // look-up (32 copies: 32 KB, o
 constexpr uint32_t kRowMask = 255u << kRowShift; // a table row is 4 * kCopies bytes
 constexpr float kCopyStep = 1.0f / kCopies;      // copy c of the table is scaled by 2^(c * kCopyStep)
 constexpr float kNoRef = 1.0e30f;                // stored negated reference of a row without one: any score exceeds it
-constexpr float kSafe = 14.0f;
+constexpr float kBelow = 10.0f, kSafe = 15.5f;   // largest exponents: in the tile that sets a reference, in any other
 constexpr int kFeeders = 2, kFeedIdBytes = 256;   // block ids: two chunks of four tiles for each feeder
 // What starting and ending a piece costs, in tiles (the share of a CTA counts it): preparing and writing out few rows is quick.
 // Chains of 16 rows: 61 us with 2, 66 with 5; trees of 64 rows: 143 us with 7, 158 with 3.
@@ -663,8 +665,8 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
                 const float old = lds_f(ref_a + 4 * (c0 + gtid));
                 float fac = 1.0f;
                 if (m + old > kSafe) {
-                  fac = old == kNoRef ? 0.f : fast_exp2(-old - m);
-                  sts_f(ref_a + 4 * (c0 + gtid), -m);
+                  fac = old == kNoRef ? 0.f : fast_exp2(kBelow - m - old);
+                  sts_f(ref_a + 4 * (c0 + gtid), kBelow - m);
                 }
                 sts_f(fac_a + 4 * (c0 + gtid), fac);
               }
