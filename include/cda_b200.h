@@ -288,6 +288,8 @@ int cda_b200_prefill_debug(int wait_limit_us, int withhold_first_k_arrive);
  *   x_n   = scale * q.k_n;  softcap > 0: softcap * tanh(x_n / softcap);  then + slope_h * (pos_n - pos_t)
  *   seen  : n < ctx, or n = ctx + j with bit j of tree_mask[t] set (no mask: j <= t); and pos_t - pos_n < window if window > 0
  *   out   = sum_n softmax(x)_n v_n over the keys seen, lse = log sum_n exp(x_n); a row that sees none: zeros, -inf
+ * A value row with a coordinate that fp16 cannot hold (a norm that is NaN, infinite or too large) makes NaN of the outputs that
+ * see its key, and of no others.
  * The position of a context key is its place, that of a new token ctx + depth, its depth being its place in a chain and
  * popcount(mask) - 1 (not below 0) in a tree.  Mask bits at and above q_len name no token: they show no key, but count for the
  * depth.

@@ -93,8 +93,9 @@ struct Cfg {
   static constexpr int kOffMax = kOffFac + 8 * NR;                // 4 warps x (kStreams x NR) floats: maxima, sums
   static constexpr int kOffCmb = kOffMax + 16 * NR * kStreams;               // 4 x NR floats: how the groups' results are put together
   static constexpr int kOffVal = kOffCmb + 16 * NR;               // 8 tiles x 128 floats: log2 of the value norms
-  static constexpr int kOffLevels = kOffVal + 4096;               // 2 x 16 floats
-  static constexpr int kOffBox = kOffLevels + 128;               // two boxes for each softmax warp
+  static constexpr int kOffBad = kOffVal + 4096;                  // 8 tiles x 128 bits: keys whose value row is not finite
+  static constexpr int kOffLevels = kOffBad + 128;                // 2 x 16 floats, and the largest of V
+  static constexpr int kOffBox = kOffLevels + 144;               // two boxes for each softmax warp
   static constexpr int kOffBar = kOffBox + 128 * kSoftWarps;                // barriers, TMEM address, wait state, plan
   static constexpr int kSmemBytes = kOffBar + kOffIds + kFeeders * kFeedIdBytes + 1024;
   static_assert(kSmemBytes <= 232448, "one CTA's shared memory");
@@ -115,6 +116,11 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {          // (not volatile: look-ups in a table that is complete)
   uint32_t v;
   asm("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
 __device__ __forceinline__ float lds_f(uint32_t a) {
@@ -194,6 +200,21 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile
     if (try_eight(bar, parity)) return true;
   ws->abort = 1;
   return false;
+}
+
+// Whether the value row of a key -- its codes at `codes` in shared memory -- holds a coordinate that fp16 cannot (it rounds what
+// is 65520 or more to infinity).  The largest level, behind the 16 levels, decides nearly always.  Such a row would make NaN of
+// the zero probabilities of the rows that do not see its key: it is taken as zeros, and the probabilities of the others are
+// made NaN.
+__device__ __forceinline__ bool row_not_finite(uint32_t codes, int bits, uint32_t levels, float norm) {
+  if (lds_f(levels + 64) * fabsf(norm) < 65520.0f) return false;
+  bool bad = false;
+#pragma unroll 1
+  for (int at = 0; at < 128 * bits; at += bits) {
+    const uint32_t code = lds_u(codes + at / 32 * 4) >> (at & 31) & ((1u << bits) - 1u);
+    bad = bad || !(fabsf(lds_f(levels + 4 * code) * norm) < 65520.0f);
+  }
+  return bad;
 }
 
 // Sums of M values per lane over the warp's 32 lanes: lane l returns the total of value l % M (M - 1 + log2(32 / M) exchanges
@@ -450,7 +471,9 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
   }
   if (tid < 32) {                                               // code levels: 16 or 4 of K, then of V
     const int side = tid >> 4, i = tid & 15, n = (side ? p.v_bits : p.k_bits) == 4 ? 16 : 4;
-    reinterpret_cast<float*>(sm + C::kOffLevels)[tid] = i < n ? __ldg((side ? p.cb_v : p.cb_k) + i) : 0.f;
+    const float level = i < n ? __ldg((side ? p.cb_v : p.cb_k) + i) : 0.f, top = warp_max(side ? fabsf(level) : 0.f);
+    reinterpret_cast<float*>(sm + C::kOffLevels)[tid] = level;
+    if (tid == 0) reinterpret_cast<float*>(sm + C::kOffLevels)[32] = top;
   }
   if (warp == C::kWarpS) {
     tmem_alloc(base + C::kOffBar + kOffTmemAddr, C::kTmemCols);
@@ -720,6 +743,18 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
 #pragma unroll
           for (int c = 0; c < C::kBlock; c += 2) sum[(c0 + c) / 2] = f2_fma(f2_pack(e[c], e[c + 1]), inv2, sum[(c0 + c) / 2]);
         }
+        if (const uint32_t bad_keys = lds_u(base + C::kOffBad + 16 * (i & 7) + 4 * (warp & 3))) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < C::kCols; c0 += 8) {            // a value row that is not finite: NaN for the rows that see the key
+            uint32_t x[8];
+            tmem_load<8>(lanes + C::kColS + (i & (C::kSBuffers - 1)) * NR + col0 + c0, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] = x[c] == 0xff800000u ? 0u : 0x7fffu;
+            if (bad_keys >> lane & 1u)
+              sts128(p_tile + sw128(key, ((col0 & 63) + c0) / 8), x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+          }
+        }
         fence_async_smem();
         tc_fence_before_sync();
         __syncwarp();
@@ -911,9 +946,12 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       } else {
         const uint2 norms = lds64(cell + norm_at);
         const bool live = key < *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage);
-        const float norm = live ? __uint_as_float(is_v ? norms.y : norms.x) : 0.f;        // keys past the end: zero rows
+        const bool bad = live && row_not_finite(cell + 16 * p.k_bits, p.v_bits, base + C::kOffLevels + 64, __uint_as_float(norms.y));
+        const float norm = !live || (is_v && bad) ? 0.f : __uint_as_float(is_v ? norms.y : norms.x);      // keys past the end: zero rows
         const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
         if (!is_v) {                                                      // (eight tiles deep: read before S of tile i + 4 is written)
+          const uint32_t bad_keys = __ballot_sync(0xffffffffu, bad);
+          if (lane == 0) *reinterpret_cast<uint32_t*>(sm + C::kOffBad + 16 * (i & 7) + 4 * (warp & 3)) = bad_keys;
           const float nv = fminf(fmaxf(__uint_as_float(norms.y), 1.0e-30f), 1.0e30f);
           sts_f(base + C::kOffVal + 4 * ((i & 7) * kKeys + key), p.v_bits == 4 && live ? __log2f(nv) - kCopyStep * static_cast<float>(key & (kCopies - 1)) : 0.f);
         }

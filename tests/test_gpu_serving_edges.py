@@ -6,7 +6,7 @@ import torch
 
 from tests import _serving as S
 from tests import _serving_exact as X
-from tests.test_gpu_serving_ops import check_mass, check_tree, run_tree
+from tests.test_gpu_serving_ops import DEV, call_args, check_mass, check_tree, on, run_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,54 @@ def test_small_terms_behind_a_dominant_key(v_bits, B, n, T):
     want, tol = X.tree_bounds(c)
     off = worst(out, want, tol)
     assert off <= 1.0, f"out is {off:.2f} bounds off"
+
+
+@pytest.mark.parametrize("k_bits,v_bits", [(4, 4), (4, 2), (2, 2), (2, 4)])
+@pytest.mark.parametrize("group", [2, 8])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, 3.0e5, 2.0e6])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(k_bits, v_bits, group, value):
+    """A NaN or infinite norm, or one whose rows come near fp16's end or beyond it, in a draft that only some rows see, and in a
+    context key behind the window: rows that do not see the key are as they would be, rows that do are NaN where its value row
+    is not finite; log-sum-exp does not know values."""
+    T = 8
+    masks = [(1 << t) | 1 for t in range(T)]                          # a root and seven siblings
+    c = S.attend_case([400, 150], [T, T], k_bits=k_bits, v_bits=v_bits, group=group, window=100, masks=masks * 2, seed=3)
+    for b, n in enumerate((400, 150)):
+        X.set_norm(c, b, n - T + 5, 1, value)                         # the sixth draft, seen by itself alone
+        X.set_norm(c, b, n - T - 101, 1, value)                       # behind every row's window
+        X.set_norm(c, b, n - T - 128 if b == 0 else 0, 1, value)
+    out, lse = run_tree(c)
+    want, tol = X.tree_bounds(c)
+    finite = torch.ones(2 * T, 2, dtype=torch.bool)                   # (row, KV head): all values that it sees are
+    for b, n in enumerate((400, 150)):
+        _, Vs = S.O.gather_sequence(c["cache"], c["block_table"][b], n, 16, k_bits, v_bits)
+        finite[b * T + 5] = S.O.decode_rotated(Vs, c["cb_V"])[0][:, n - T + 5].isfinite().all(-1)
+    assert bool(finite[5].all()) == (value == 3.0e5)                  # (rows of encoded values: levels up to 0.21 of the norm)
+    seen = finite.repeat_interleave(group, 1)
+    assert worst(out, want, tol, seen) <= 1.0
+    assert not bool(out.cpu()[~seen].isfinite().any())
+    _, _, wz, ztol = S.tree_reference(c)
+    assert float(((lse.double().cpu() - wz).abs() / ztol).max()) <= 1.0
+
+
+@pytest.mark.parametrize("k_bits", [4, 2])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_keys_that_are_not_finite_reach_the_rows_that_see_them(k_bits, value):
+    from sub0_b200 import ops
+    T = 6
+    masks = [(1 << t) | 1 for t in range(T)]
+    c = S.attend_case([300], [T], k_bits=k_bits, masks=masks, seed=4)
+    want, tol = X.tree_bounds(c)                                      # of the other rows, which do not see the fourth draft
+    z = S.tree_reference(c)[2].float()
+    X.set_norm(c, 0, 300 - T + 3, 0, value)
+    out, lse = run_tree(c)
+    rest = [t for t in range(T) if t != 3]
+    assert worst(out, want, tol, rest) <= 1.0 and not bool(out[3].isfinite().any())
+    z[3] = 0.0
+    weights = torch.ones(T)
+    mass = torch.zeros(1, 2, 300, device=DEV)
+    ops.attention_mass(on(c["Q"]), on(c["cache"]), on(c["block_table"]), on(c["seq_lens"]), on(z), mass, weights=on(weights), **call_args(c))
+    assert ops.kv_status() == 0
+    bad = torch.zeros(300, dtype=torch.bool)
+    bad[300 - T + 3] = True
+    assert bool(mass[..., ~bad].isfinite().all())
