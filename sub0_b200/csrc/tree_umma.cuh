@@ -23,12 +23,15 @@
 // down to 2^-24 of the largest (17 nats below it) in fp16's normal range: where one key draws nearly all attention and has a
 // small value row, they are the output.  (With the reference at the maximum, such an output of 1500 keys was off by 2 %.)
 //
-// Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 129 us (slots: 20 us at copy
-// bandwidth); one tree of 32 x 4 rows over 131k keys 209 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 705 us, 390
-// TFLOP/s.  What bounds it: blocks of up to 64 rows wait for the producers -- a tile takes the V group 3700 cycles, of which 2400
-// are its look-ups, and each K group 7500 for every second tile, while the tensor cores are busy 18% of the time; blocks of 128
-// rows for the softmax (a chain of some 4500 cycles a tile) and for the clock that the power limit leaves.  A new piece costs 12 to 16 us beside
-// its tiles: query rows, references, the way back, in code that has to come out of L2.
+// Both sides' rows are the format's own, fp16(level * norm), from byte permutes of a key's 16 (or 4) values.  (4-bit value rows from
+// a table of fp16 levels, with the norm on the probability, are rounded in another way and 7 us of 138 faster in the batch below.)
+//
+// Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 145 us (slots: 20 us at copy
+// bandwidth); one tree of 32 x 4 rows over 131k keys 213 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 755 us, 364
+// TFLOP/s.  What bounds it: blocks of up to 64 rows wait for the producers -- the V group takes some 4100 cycles a tile, which is
+// the pace; each K group has twice that for every second tile -- while the tensor cores are busy 16% of the time; blocks of 128
+// rows for the softmax (a chain of some 4800 cycles a tile) and for the clock that the power limit leaves.  A new piece costs 12 to
+// 16 us beside its tiles: query rows, references, the way back, in code that has to come out of L2.
 #pragma once
 #include "attend.cuh"
 #include "cache_map.cuh"
@@ -43,10 +46,6 @@ using namespace umma;
 constexpr int kKeys = 128, kTileBytes = 32768, kColBlock = 16384;
 constexpr int kStageBytes = kKeys * 144;         // 128 slots side by side; their widths (144, 112, 80) are odd multiples of 16,
                                                  // so threads that read the same piece of 8 neighbouring slots meet no conflict
-constexpr int kCopies = 8;                       // of the value table, one for every four lanes: 8 KB and about two wavefronts a
-constexpr int kRowShift = 5;                     // look-up (32 copies: 32 KB, one wavefront, and one ring stage less)
-constexpr uint32_t kRowMask = 255u << kRowShift; // a table row is 4 * kCopies bytes
-constexpr float kCopyStep = 1.0f / kCopies;      // copy c of the table is scaled by 2^(c * kCopyStep)
 constexpr float kNoRef = 1.0e30f;                // stored negated reference of a row without one: any score exceeds it
 constexpr float kBelow = 10.0f, kSafe = 15.5f;   // largest exponents: in the tile that sets a reference, in any other
 constexpr int kFeeders = 2, kFeedIdBytes = 256;   // block ids: two chunks of four tiles for each feeder
@@ -84,22 +83,19 @@ struct Cfg {
   // shared memory (bytes from a 1024-aligned base)
   static constexpr int kOffV = 0, kOffP = 2 * kTileBytes, kOffQ = kOffP + 2 * kColBlock,   // P: one of 64 rows for each stream, or one of 128
                         kOffRing = kOffQ + NR * 512;
-  static constexpr int kOffTab = kOffRing + kRing * kStageBytes;  // code byte -> two fp16 levels of V, kCopies times
-  static constexpr int kOffRef = kOffTab + 1024 * kCopies;                 // words of the rows, of two pieces in turn: negated references
+  static constexpr int kOffRef = kOffRing + kRing * kStageBytes;  // words of the rows, of two pieces in turn: negated references
   static constexpr int kOffPos = kOffRef + 16 * NR;               //   (of both groups), position,
   static constexpr int kOffSlope = kOffPos + 8 * NR;              //   slope x log2 e,
   static constexpr int kOffMask = kOffSlope + 8 * NR;             //   64-bit ancestor mask
   static constexpr int kOffFac = kOffMask + 16 * NR;              // 2 x NR floats: factors of a slow path
   static constexpr int kOffMax = kOffFac + 8 * NR;                // 4 warps x (kStreams x NR) floats: maxima, sums
   static constexpr int kOffCmb = kOffMax + 16 * NR * kStreams;               // 4 x NR floats: how the groups' results are put together
-  static constexpr int kOffVal = kOffCmb + 16 * NR;               // 8 tiles x 128 floats: log2 of the value norms
-  static constexpr int kOffBad = kOffVal + 4096;                  // 8 tiles x 128 bits: keys whose value row is not finite
+  static constexpr int kOffBad = kOffCmb + 16 * NR;               // 8 tiles x 128 bits: keys whose value row is not finite
   static constexpr int kOffLevels = kOffBad + 128;                // 2 x 16 floats, and the largest of V
   static constexpr int kOffBox = kOffLevels + 144;               // two boxes for each softmax warp
   static constexpr int kOffBar = kOffBox + 128 * kSoftWarps;                // barriers, TMEM address, wait state, plan
   static constexpr int kSmemBytes = kOffBar + kOffIds + kFeeders * kFeedIdBytes + 1024;
   static_assert(kSmemBytes <= 232448, "one CTA's shared memory");
-  static_assert(8 * (kThreads / 32) <= 1024 * kCopies, "the prologue's scan words fit the table's");
 };
 
 // ---- shared memory access -----------------------------------------------------------------------------------------------
@@ -480,7 +476,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     tmem_relinquish();
   }
   tc_fence_before_sync();
-  find_share<NR, C::kThreads>(p, reinterpret_cast<int2*>(sm + C::kOffTab), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kOffPlanEnd));
+  find_share<NR, C::kThreads>(p, reinterpret_cast<int2*>(sm + C::kOffP), s_plan, reinterpret_cast<int*>(sm + C::kOffBar + kOffPlanEnd));
   tc_fence_after_sync();
   const int total = s_plan[3];
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + C::kOffBar + kOffTmemAddr);
@@ -660,8 +656,6 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
           tmem_load<C::kBlock>(lanes + C::kColS + (i & (C::kSBuffers - 1)) * NR + col0, s);      // instead of the raw ones
         }
         const uint64_t ff = f2_pack(finish ? 1.0f : kf, finish ? 1.0f : kf);
-        // the norm of a 4-bit value row rides on the probability: P = exp2(x + log2 norm - reference), p = P / norm
-        const float lg = lds_f(base + C::kOffVal + 4 * ((i & 7) * kKeys + key));
         const uint32_t p_tile = base + C::kOffP + (C::kStreams == 2 ? stream : col0 >> 6) * kColBlock;
 #pragma unroll
         for (int blk = 0; blk < C::kCols / C::kBlock; ++blk) {
@@ -676,7 +670,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
               float top = 0.f;
 #pragma unroll
               for (int c = 0; c < C::kBlock; ++c) {
-                const float m = warp_max(fmaf(__uint_as_float(s[c]), finish ? 1.0f : kf, lg));
+                const float m = warp_max(__uint_as_float(s[c]) * (finish ? 1.0f : kf));
                 top = lane == c ? m : top;
               }
               if (lane < C::kBlock) sts_f(max_a + 4 * ((warp & 3) * C::kCols + lane), top);
@@ -697,13 +691,12 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
             }
             // probabilities against the references as they are; `excess`: the largest exponent
             float excess = -INFINITY;
-            const uint64_t lg2 = f2_pack(lg, lg);
 #pragma unroll
             for (int c = 0; c < C::kBlock; c += 4) {
               const uint4 r = lds128(ref_a + 4 * (c0 + c));
               float* a = e + c;
-              f2_unpack(f2_fma(f2_pack(s[c], s[c + 1]), ff, f2_add(f2_pack(r.x, r.y), lg2)), a[0], a[1]);
-              f2_unpack(f2_fma(f2_pack(s[c + 2], s[c + 3]), ff, f2_add(f2_pack(r.z, r.w), lg2)), a[2], a[3]);
+              f2_unpack(f2_fma(f2_pack(s[c], s[c + 1]), ff, f2_pack(r.x, r.y)), a[0], a[1]);
+              f2_unpack(f2_fma(f2_pack(s[c + 2], s[c + 3]), ff, f2_pack(r.z, r.w)), a[2], a[3]);
               excess = fmax3(excess, a[0], a[1]);
               excess = fmax3(excess, a[2], a[3]);
 #pragma unroll
@@ -738,10 +731,8 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
             }
             if (!group_any(group, excess > kSafe)) break;
           }
-          const float inv = fast_exp2(-lg);
-          const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
-          for (int c = 0; c < C::kBlock; c += 2) sum[(c0 + c) / 2] = f2_fma(f2_pack(e[c], e[c + 1]), inv2, sum[(c0 + c) / 2]);
+          for (int c = 0; c < C::kBlock; c += 2) sum[(c0 + c) / 2] = f2_add(sum[(c0 + c) / 2], f2_pack(e[c], e[c + 1]));
         }
         if (const uint32_t bad_keys = lds_u(base + C::kOffBad + 16 * (i & 7) + 4 * (warp & 3))) {
 #pragma unroll 1
@@ -903,16 +894,6 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     const uint32_t cell0 = base + C::kOffRing + key * p.slot_bytes, code_at = is_v ? 16 * p.k_bits : 0;
     const uint32_t norm_at = 16 * (p.k_bits + p.v_bits), row0 = base + C::kOffV;
     const float* levels = reinterpret_cast<const float*>(sm + C::kOffLevels) + (is_v ? 16 : 0);
-    const uint32_t tab_a = base + C::kOffTab + 4 * (lane & (kCopies - 1));
-    if (is_v && bits == 4) {
-      // The V warps fill the value table.  Copy c holds the levels times 2^(c / 8), its keys' norms the inverse: a level's rounding
-      // to fp16 would else be the same for every key, a bias that stays while the outputs of a long context average out (131k keys:
-      // error against 64 bits 7.3e-4 of the output with equal copies)
-      for (int k = tid - C::kWarpV * 32; k < 256 * kCopies; k += 128) {
-        const float by = exp2f(kCopyStep * static_cast<float>(k & (kCopies - 1)));
-        *reinterpret_cast<uint32_t*>(sm + C::kOffTab + 4 * k) = pack_half2(levels[k / (16 * kCopies)] * by, levels[(k / kCopies) & 15] * by);
-      }
-    }
     const int id = is_v ? 6 : 7 + begin;                        // named barriers: V 6; K 7, 8
     int stage = begin, wraps = 0;                               // of the ring
 #pragma unroll 1
@@ -926,51 +907,30 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       named_barrier(id, 128);
       tc_fence_after_sync();
       const uint32_t cell = cell0 + stage * kStageBytes;
-      if (is_v && bits == 4) {
-        // 4-bit values: fp16 levels from the table, one look-up per code byte; the norm goes into the key's probabilities
+      const uint2 norms = lds64(cell + norm_at);
+      const bool live = key < *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage);
+      const bool bad = live && row_not_finite(cell + 16 * p.k_bits, p.v_bits, base + C::kOffLevels + 64, __uint_as_float(norms.y));
+      const float norm = !live || (is_v && bad) ? 0.f : __uint_as_float(is_v ? norms.y : norms.x);      // keys past the end: zero rows
+      const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
+      if (!is_v) {                                                      // (eight tiles deep: read before S of tile i + 4 is written)
+        const uint32_t bad_keys = __ballot_sync(0xffffffffu, bad);
+        if (lane == 0) *reinterpret_cast<uint32_t*>(sm + C::kOffBad + 16 * (i & 7) + 4 * (warp & 3)) = bad_keys;
+      }
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          const uint4 w4 = lds128(cell + code_at + 16 * c);
-          const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w}, to = row + (c >> 1) * kColBlock;
-          uint32_t v[16];                                       // all look-ups first: a store in between would wait for each
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            v[4 * u] = lds32(tab_a + ((ws[u] << kRowShift) & kRowMask));
-            v[4 * u + 1] = lds32(tab_a + ((ws[u] >> (8 - kRowShift)) & kRowMask));
-            v[4 * u + 2] = lds32(tab_a + ((ws[u] >> (16 - kRowShift)) & kRowMask));
-            v[4 * u + 3] = lds32(tab_a + ((ws[u] >> (24 - kRowShift)) & kRowMask));
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) sts128(to + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+      for (int c = 0; c < 4; ++c) {                                     // 32 coordinates at a time
+        uint32_t v[16];
+        if (bits == 4) {
+          expand::quarter4(t, lds128(cell + code_at + 16 * c), v);
+        } else {
+          const uint2 w = lds64(cell + code_at + 8 * c);
+          expand::quarter2(t, w.x, w.y, v);
         }
-      } else {
-        const uint2 norms = lds64(cell + norm_at);
-        const bool live = key < *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage);
-        const bool bad = live && row_not_finite(cell + 16 * p.k_bits, p.v_bits, base + C::kOffLevels + 64, __uint_as_float(norms.y));
-        const float norm = !live || (is_v && bad) ? 0.f : __uint_as_float(is_v ? norms.y : norms.x);      // keys past the end: zero rows
-        const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
-        if (!is_v) {                                                      // (eight tiles deep: read before S of tile i + 4 is written)
-          const uint32_t bad_keys = __ballot_sync(0xffffffffu, bad);
-          if (lane == 0) *reinterpret_cast<uint32_t*>(sm + C::kOffBad + 16 * (i & 7) + 4 * (warp & 3)) = bad_keys;
-          const float nv = fminf(fmaxf(__uint_as_float(norms.y), 1.0e-30f), 1.0e30f);
-          sts_f(base + C::kOffVal + 4 * ((i & 7) * kKeys + key), p.v_bits == 4 && live ? __log2f(nv) - kCopyStep * static_cast<float>(key & (kCopies - 1)) : 0.f);
-        }
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {                                     // 32 coordinates at a time
-          uint32_t v[16];
-          if (bits == 4) {
-            expand::quarter4(t, lds128(cell + code_at + 16 * c), v);
-          } else {
-            const uint2 w = lds64(cell + code_at + 8 * c);
-            expand::quarter2(t, w.x, w.y, v);
-          }
-          if (is_v) {
+        if (is_v) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              sts128(row + (c >> 1) * kColBlock + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-          } else {
-            tmem_st16(lanes + buffer * 64 + 16 * c, v);
-          }
+          for (int u = 0; u < 4; ++u)
+            sts128(row + (c >> 1) * kColBlock + sw128(key, (c & 1) * 4 + u), v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        } else {
+          tmem_st16(lanes + buffer * 64 + 16 * c, v);
         }
       }
       if (is_v) fence_async_smem();

@@ -56,6 +56,27 @@ def test_small_terms_behind_a_dominant_key(v_bits, B, n, T):
     assert off <= 1.0, f"out is {off:.2f} bounds off"
 
 
+@pytest.mark.parametrize("k_bits,v_bits", [(4, 4), (4, 2), (2, 4), (2, 2)])
+@pytest.mark.parametrize("group", [1, 4, 8])
+def test_value_rows_are_the_formats(k_bits, v_bits, group):
+    """Rows that see a single key give its value row fp16(level * norm), rotated back: rounded once, when it is written."""
+    c = S.attend_case([64, 1, 33], [64, 1, 33], k_bits=k_bits, v_bits=v_bits, group=group, seed=group, masks=[1 << t for n in (64, 1, 33) for t in range(n)])
+    out, _ = run_tree(c)
+    want, tol = X.tree_bounds(c, own=True)
+    off = worst(out, want, tol)
+    assert off <= 1.0, f"out is {off:.2f} bounds off"
+
+
+@pytest.mark.parametrize("name", ["ragged, empty sequence", "drafts across a tile", "group 8, 512 rows", "long chain", "all modifiers", "k2v4, page 32"])
+def test_tree_attention_within_the_formats_bound(name):
+    from tests.test_gpu_serving_ops import TREES
+    c = S.attend_case(seed=len(name), **TREES[name])
+    out, _ = run_tree(c)
+    want, tol = X.tree_bounds(c)
+    off = worst(out, want, tol)
+    assert off <= 1.0, f"out is {off:.2f} bounds off"
+
+
 @pytest.mark.parametrize("k_bits,v_bits", [(4, 4), (4, 2), (2, 2), (2, 4)])
 @pytest.mark.parametrize("group", [2, 8])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, 3.0e5, 2.0e6])
