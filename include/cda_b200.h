@@ -346,7 +346,7 @@ int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table, const int
  * slot);  bit 2 (4) a bounded wait gave up and rows were left unwritten;  bit 3 (8) lengths that do not fit the call;
  * bit 4 (16) a refused entry of a keep list or a negative start.  Negative status on a CUDA error. */
 int cda_b200_kv_status(void);
-int cda_b200_kv_clear_status(void);
+int cda_b200_kv_clear_status(void);   /* (synchronises the device: calls made before it do not report after it) */
 
 #ifdef __cplusplus
 }

@@ -372,15 +372,17 @@ extern "C" int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table
                            : launch_clusters("compact_cache", compact_cache_kernel<5>, rows, ranks, kCompactThreads, 0, st, p);
 }
 
+// The copies below run on the legacy default stream, which non-blocking streams neither wait for nor are waited for by: the
+// device is synchronised first, so that every call made before has reported.
 extern "C" int cda_b200_kv_status(void) {
   int v = 0, t = 0;
-  if (cudaMemcpyFromSymbol(&v, g_evict_status, sizeof(int)) != cudaSuccess) return check_launch("kv_status");
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&v, g_evict_status, sizeof(int)) != cudaSuccess) return check_launch("kv_status");
   const int rc = tree_status(false, &t);
   return rc != CDA_OK ? rc : (v | t) & 0x7fffffff;
 }
 
 extern "C" int cda_b200_kv_clear_status(void) {
   const int zero = 0;
-  if (cudaMemcpyToSymbol(g_evict_status, &zero, sizeof(int)) != cudaSuccess) return check_launch("kv_clear_status");
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyToSymbol(g_evict_status, &zero, sizeof(int)) != cudaSuccess) return check_launch("kv_clear_status");
   return tree_status(true, nullptr);
 }

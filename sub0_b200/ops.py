@@ -600,4 +600,5 @@ def kv_status() -> int:
 
 
 def kv_clear_status() -> None:
+    """Clears the bits of :func:`kv_status`.  Synchronises the device."""
     check(lib.cda_b200_kv_clear_status())

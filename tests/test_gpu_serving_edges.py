@@ -126,3 +126,43 @@ def test_keys_that_are_not_finite_reach_the_rows_that_see_them(k_bits, value):
     bad = torch.zeros(300, dtype=torch.bool)
     bad[300 - T + 3] = True
     assert bool(mass[..., ~bad].isfinite().all())
+
+
+# ---- limits and status ------------------------------------------------------------------------------------------------
+
+def busy(milliseconds=60):
+    torch.cuda._sleep(int(milliseconds * 1.9e6))
+
+
+def test_status_waits_for_other_streams():
+    """A call on a side stream, still queued behind long work, has reported by the time its status is read, and a status that
+    is cleared stays clear of it."""
+    from sub0_b200 import ops
+    c = S.attend_case([50, 60], [5, 4], seed=1)
+    sl = c["seq_lens"].clone()
+    sl[1] = 3
+    dev = [on(c["Q"]), on(c["cache"]), on(c["block_table"]), on(sl)]
+    out, a, cb_V = torch.empty_like(dev[0]), call_args(c), on(c["cb_V"])
+    mass = torch.rand(1, 1, 20, device=DEV)
+    long = on(torch.tensor([25], dtype=torch.int32))
+    side = torch.cuda.Stream()
+    calls = (lambda: ops.tree_attention(*dev, out, cb_V=cb_V, **a), lambda: ops.select_keys(mass, long, 8))
+    for call in calls:                                                # (once, so that nothing is loaded behind the busy stream)
+        call()
+    assert ops.kv_status() == ops.KV_LENGTHS
+    ops.kv_clear_status()
+    for call in calls:
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            busy()
+            call()
+        assert ops.kv_status() == ops.KV_LENGTHS
+        ops.kv_clear_status()
+        assert ops.kv_status() == 0
+        with torch.cuda.stream(side):
+            busy()
+            call()
+        ops.kv_clear_status()
+        torch.cuda.synchronize()
+        assert ops.kv_status() == 0
+    ops.kv_clear_status()
