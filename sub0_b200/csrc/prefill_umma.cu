@@ -825,25 +825,28 @@ int dispatch_prefill_umma(const PrefillUmmaParams& p, int k_bits, int v_bits, in
 
 }  // namespace cda
 
+// The copies below run on the legacy default stream, which does not wait for non-blocking streams: the device is synchronised
+// first.
+//
 // 1 if a prefill CTA on the current device gave up on a wait since the last clear (synchronises the device), 0 if not,
 // < 0 on error.
 extern "C" int cda_b200_prefill_fault(void) {
   int v = 0;
-  if (cudaMemcpyFromSymbol(&v, cda::g_prefill_fault, sizeof(int)) != cudaSuccess) return cda::check_launch("prefill_fault");
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&v, cda::g_prefill_fault, sizeof(int)) != cudaSuccess) return cda::check_launch("prefill_fault");
   return v != 0 ? 1 : 0;
 }
 
 // Status bits the prefill kernel raised on the current device since the last clear (synchronises the device).
 extern "C" int cda_b200_prefill_status(void) {
   int v = 0;
-  if (cudaMemcpyFromSymbol(&v, cda::g_prefill_status, sizeof(int)) != cudaSuccess) return cda::check_launch("prefill_status");
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&v, cda::g_prefill_status, sizeof(int)) != cudaSuccess) return cda::check_launch("prefill_status");
   return v & 0x7fffffff;
 }
 
 // Clears the status bits and the fault flag of the current device (synchronises the device).
 extern "C" int cda_b200_prefill_clear_status(void) {
   const int zero = 0;
-  if (cudaMemcpyToSymbol(cda::g_prefill_status, &zero, sizeof(int)) != cudaSuccess ||
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyToSymbol(cda::g_prefill_status, &zero, sizeof(int)) != cudaSuccess ||
       cudaMemcpyToSymbol(cda::g_prefill_fault, &zero, sizeof(int)) != cudaSuccess)
     return cda::check_launch("prefill_clear_status");
   return CDA_OK;

@@ -166,3 +166,32 @@ def test_status_waits_for_other_streams():
         torch.cuda.synchronize()
         assert ops.kv_status() == 0
     ops.kv_clear_status()
+
+
+def test_prefill_status_waits_for_other_streams():
+    from sub0_b200 import ops
+    from tests import _cases as Cs
+    from tests.test_gpu_prefill import prefill_inputs
+    case = Cs.paged_case([70], H_kv=1, group=4, seed=2)
+    Q, cu = prefill_inputs(case, [5], 3)
+    out = torch.empty_like(Q, device=DEV)
+    dev = [on(Q), on(case["cache"]), on(case["block_table"]), on(cu), on(torch.tensor([3], dtype=torch.int32)), out]
+    cb_K, cb_V = on(case["cb_K"]), on(case["cb_V"])
+    call = lambda: ops.prefill_varlen(*dev, cb_K=cb_K, cb_V=cb_V, block_size=16, max_query_len=5, max_seq_len=70)  # noqa: E731
+    call()
+    assert ops.prefill_status() == ops.PREFILL_QLEN_EXCEEDS_SEQLEN
+    ops.prefill_clear_status()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        busy()
+        call()
+    assert ops.prefill_status() == ops.PREFILL_QLEN_EXCEEDS_SEQLEN
+    ops.prefill_clear_status()
+    assert ops.prefill_status() == 0
+    with torch.cuda.stream(side):
+        busy()
+        call()
+    ops.prefill_clear_status()
+    torch.cuda.synchronize()
+    assert ops.prefill_status() == 0 and ops.prefill_fault() is False
