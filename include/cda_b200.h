@@ -334,7 +334,8 @@ int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, int32_t* ke
  * Every entry must satisfy start[b] + i <= keep < seq_lens[b]; a negative one leaves its destination as it is, one that
  * breaks the rule is skipped and reported (cda_b200_kv_status).  keep (B, keep_heads, K) int32, keep_heads = H_kv or 1 (one
  * list for all heads).  With `mass` (B, H_kv, mass_stride) the weights move along: a destination gets its key's weight (0
- * without a valid entry), and those from start + K to the end of the sequence become 0.  The pages that a sequence writes to
+ * where no slot comes to it: a negative or refused entry, a block outside the cache), and those from start + K to the end of the
+ * sequence become 0.  The pages that a sequence writes to
  * must be its own: a page that two block tables share is moved for both.  Slots behind the moved ones keep their bytes.
  * No counterpart in the reference. */
 int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table, const int32_t* seq_lens, const int32_t* keep,

@@ -273,8 +273,9 @@ __global__ void __launch_bounds__(kCompactThreads, 4) compact_cache_kernel(const
         atomicOr(&g_evict_status, kStatusKeep);
       } else if (src >= 0) {
         from = slot(src);
-        to = from >= 0 && src != dst ? slot(static_cast<int>(dst)) : -1;
-        if (mass && src < p.mass_stride) m = mass[src];
+        to = from < 0 ? -1 : src != dst ? slot(static_cast<int>(dst)) : from;
+        if (mass && to >= 0 && src < p.mass_stride) m = mass[src];      // a weight goes where its slot goes
+        if (src == dst) to = -1;                  // (it stays)
       }
     }
     s_from[tid] = to >= 0 ? from : -1;

@@ -561,7 +561,7 @@ def compact_cache(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, keep:
     ``start``).  ``keep`` (B, H_kv or 1, K) int32; every entry satisfies ``start[b] + i <= keep < seq_lens[b]`` or is negative,
     which leaves its destination as it is.  After :func:`select_keys` this shortens the sequences to its ``new_lens``; with
     ``start`` = the context's length and ``keep`` = the accepted path it moves accepted drafts behind the context.  ``mass``
-    moves along, and becomes 0 from ``start + K`` to the sequence's end.  The pages written to must belong to one sequence."""
+    moves along, and becomes 0 where no slot comes to a destination and from ``start + K`` to the sequence's end.  The pages written to must belong to one sequence."""
     _cuda(kv_cache, "kv_cache")
     dev = kv_cache.device
     _same_device(dev, block_table=block_table, seq_lens=seq_lens, keep=keep, start=start, mass=mass)

@@ -6,7 +6,7 @@ import torch
 
 from tests import _serving as S
 from tests import _serving_exact as X
-from tests.test_gpu_serving_ops import DEV, call_args, check_mass, check_tree, on, run_tree
+from tests.test_gpu_serving_ops import DEV, call_args, check_mass, check_tree, compact_case, on, run_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -195,3 +195,37 @@ def test_prefill_status_waits_for_other_streams():
     ops.prefill_clear_status()
     torch.cuda.synchronize()
     assert ops.prefill_status() == 0 and ops.prefill_fault() is False
+
+
+# ---- selection and compaction -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_compaction_skips_bad_blocks_with_their_weights(shared):
+    """Slots whose block, at either end of the move, lies outside the cache stay as they are; a place that no slot came to has the
+    weight 0."""
+    from sub0_b200 import ops
+    cache, table, lens, keep, _, mass = compact_case([600, 300], 200, seed=8, shared=shared)
+    bad = table.clone()
+    bad[0, 3], bad[0, 20], bad[1, 0], bad[1, 9] = 1 << 30, -1, cache.shape[0] // 16, -7
+    keep[0, 0, :5] = torch.arange(5, dtype=torch.int32)               # slots that stay where they are: in a good block,
+    keep[1, 0, :5] = torch.arange(5, dtype=torch.int32)               # in a bad one
+    want, want_mass = cache.clone(), mass.clone()
+    ok = lambda b, t: 0 <= int(bad[b, t // 16]) < cache.shape[0] // 16  # noqa: E731
+    place = lambda b, t: int(bad[b, t // 16]) * 16 + t % 16  # noqa: E731
+    for b in range(2):
+        for h in range(2):
+            for i in range(200):
+                src = int(keep[b, 0 if shared else h, i])
+                moved = src >= 0 and ok(b, src) and ok(b, i)
+                if moved:
+                    want[place(b, i), h] = cache[place(b, src), h]
+                want_mass[b, h, i] = mass[b, h, src] if moved else 0.0
+            want_mass[b, h, 200:int(lens[b])] = 0.0
+    for with_mass in (True, False):
+        got, got_mass = on(cache), on(mass) if with_mass else None
+        ops.compact_cache(got, on(bad), on(lens), on(keep), block_size=16, mass=got_mass)
+        assert ops.kv_status() == ops.KV_BAD_BLOCK
+        ops.kv_clear_status()
+        assert torch.equal(got.cpu(), want)
+        if with_mass:
+            assert torch.equal(got_mass.cpu(), want_mass)
