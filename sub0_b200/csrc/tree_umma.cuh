@@ -259,6 +259,9 @@ __device__ __forceinline__ Entry entry_of(const AttendParams& p, int e) {
   x.tiles = (hi + kKeys - 1) / kKeys - x.first;
   return x;
 }
+// An entry without tiles is behind its sequence's last row: so are those up to the next sequence.  (A call that allows far more new
+// tokens than a sequence brings has hundreds of thousands of them, longer to step through than a wait may take.)
+__device__ __forceinline__ int after_empty(const AttendParams& p, int b) { return (b + 1) * p.row_blocks; }
 struct Piece { Entry x; int e, head, tile0, n; bool starts, ends; };
 // What a softmax warp needs of a piece at its start and end, and where its walk stands, in shared memory (a box for each warp):
 // held in registers they were spilled, and every start and end of a piece waited for L2 (1024 threads' stacks fit no L1).
@@ -269,7 +272,7 @@ struct Walk {
   __device__ __forceinline__ bool next(const AttendParams& p, Piece& q) {
     while (left > 0 && e < entries) {
       q.x = entry_of<NR>(p, e);
-      if (q.x.tiles == 0) { ++e; continue; }
+      if (q.x.tiles == 0) { e = after_empty(p, q.x.b); continue; }
       q.e = e; q.head = h;
       q.tile0 = q.x.first + j;
       q.n = min(left, q.x.tiles - j);
@@ -306,13 +309,14 @@ struct Space {
 template <int NR, int THREADS>
 __device__ __forceinline__ void find_share(const AttendParams& p, int2* s_scan, int* s_plan, int* s_end) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, entries = p.B * p.row_blocks;
-  const int per = (entries + THREADS - 1) / THREADS, e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
+  const int per = (entries + THREADS - 1) / THREADS, e0 = min(tid * per, entries), e1 = e0 + min(per, entries - e0);
   int tiles = 0, used = 0;                                       // of this thread's entries, one head: tiles, entries with any
-  for (int e = e0; e < e1; ++e) {
-    const int n = entry_of<NR>(p, e).tiles;
-    tiles += n;
-    used += n > 0;
-    if (blockIdx.x == 0 && e % p.row_blocks == 0 && sequence_view(p, e / p.row_blocks).bad) atomicOr(&g_tree_status, kStatusLengths);
+  for (int e = e0; e < e1;) {
+    const Entry x = entry_of<NR>(p, e);
+    tiles += x.tiles;
+    used += x.tiles > 0;
+    if (blockIdx.x == 0 && x.rb == 0 && sequence_view(p, x.b).bad) atomicOr(&g_tree_status, kStatusLengths);
+    e = x.tiles > 0 ? e + 1 : after_empty(p, x.b);
   }
   int x = tiles, y = used;
 #pragma unroll
@@ -336,8 +340,10 @@ __device__ __forceinline__ void find_share(const AttendParams& p, int2* s_scan, 
   const int64_t mine = (tiles + static_cast<int64_t>(kPieceCost<NR>) * used) * p.H_kv;
   if (hi > lo && hi > at && lo < at + mine) {                    // the line's positions lo or hi - 1 may lie in these entries
     int real = tiles_before * p.H_kv;
-    for (int e = e0; e < e1; ++e) {
-      const int n = entry_of<NR>(p, e).tiles, len = n + kPieceCost<NR>;
+    for (int e = e0, after; e < e1; e = after) {
+      const Entry x = entry_of<NR>(p, e);
+      const int n = x.tiles, len = n + kPieceCost<NR>;
+      after = n > 0 ? e + 1 : after_empty(p, x.b);
       if (n == 0) continue;
       const int64_t next = at + static_cast<int64_t>(len) * p.H_kv;
       if (at <= lo && lo < next) {

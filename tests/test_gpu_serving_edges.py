@@ -130,6 +130,14 @@ def test_keys_that_are_not_finite_reach_the_rows_that_see_them(k_bits, value):
 
 # ---- limits and status ------------------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("max_q", [1 << 16, 1 << 23])
+def test_query_limits_far_above_the_chunks(max_q):
+    """Hundreds of short sequences under a limit that would allow each of them hundreds of thousands of row blocks."""
+    c = S.attend_case([40] * 250 + [300], [1] * 250 + [40], H_kv=1, group=8, tree=False, seed=2)
+    out, lse = run_tree(c, max_query_len=max_q)
+    check_tree(c, out, lse)
+
+
 def busy(milliseconds=60):
     torch.cuda._sleep(int(milliseconds * 1.9e6))
 
