@@ -237,3 +237,20 @@ def test_compaction_skips_bad_blocks_with_their_weights(shared):
         assert torch.equal(got.cpu(), want)
         if with_mass:
             assert torch.equal(got_mass.cpu(), want_mass)
+
+
+# ---- backend ----------------------------------------------------------------------------------------------------------
+
+def test_backend_caps_scores_of_long_prompts_beside_decodes():
+    from sub0_b200.vllm_integration.cda_attn_v2 import get_backend_classes
+    from tests.test_gpu_vllm_backend import metadata, vllm_cache
+    _, Impl, _, Metadata = get_backend_classes()
+    q_lens = [1, 1, 700, 300]
+    c = S.attend_case([900, 33, 700, 650], q_lens, tree=False, softcap=15.0, seed=23)
+    impl = Impl(8, 128, c["scale"], num_kv_heads=2, logits_soft_cap=15.0)
+    md, _ = metadata(Metadata, q_lens, c)
+    n = sum(q_lens)
+    out = torch.full((n, 1024), float("nan"), dtype=torch.float16, device=DEV)
+    impl.forward(None, on(c["Q"]).view(n, -1), None, None, vllm_cache(c), md, output=out)
+    want, tol = X.tree_bounds(c)
+    assert worst(out.view(n, 8, 128), want, tol) <= 1.0
