@@ -349,6 +349,11 @@ int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table, const int
 int cda_b200_kv_status(void);
 int cda_b200_kv_clear_status(void);   /* (synchronises the device: calls made before it do not report after it) */
 
+/* Diagnostic knobs for the tree_attention and attention_mass launches that follow in this process: the limit of every in-kernel
+ * wait in microseconds (<= 0: the default, 50 ms) and, if withhold_first_k_arrive != 0, CTA 0 waits for a signal more of its
+ * first K tile than it gets, so that the waits run out: its rows or weights stay as they were, and cda_b200_kv_status reports bit 2. */
+int cda_b200_kv_debug(int wait_limit_us, int withhold_first_k_arrive);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,7 @@ PROTOTYPES = {
     "cda_b200_compact_cache": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _i64, _i, _p]),
     "cda_b200_kv_status": (_i, []),
     "cda_b200_kv_clear_status": (_i, []),
+    "cda_b200_kv_debug": (_i, [_i, _i]),
 }
 
 

@@ -32,7 +32,11 @@ struct AttendParams {
   uint32_t group_magic;          // ceil(2^32 / group): row / group = umulhi(row, magic) for rows below 2^26
   float scale, softcap;          // softcap 0: none
   int window;                    // 0: none
+  int withhold;                  // diagnostic: CTA 0 waits for a signal too many of its first K tile
+  unsigned long long wait_limit_ns;
 };
+
+__device__ __forceinline__ int withheld(const AttendParams& p, int k_buffer) { return p.withhold && k_buffer == 0 && blockIdx.x == 0; }
 
 // The lengths of sequence b; q_len = 0 when there is nothing to do or the lengths do not fit the call (`bad`).
 struct SequenceView { int q_begin, q_len, seq_len; bool bad; };

@@ -165,13 +165,13 @@ __global__ void __launch_bounds__(MassCfg<NR>::kThreads, 1) attention_mass_kerne
   auto bar = [&](int i) { return bar0 + 8u * i; };
 
   if (tid == 0) {
-    for (int i = 0; i < C::kKGroups; ++i) { mbar_init(bar(kMKFull + i), 4); mbar_init(bar(kMKEmpty + i), 1); }
+    for (int i = 0; i < C::kKGroups; ++i) { mbar_init(bar(kMKFull + i), 4 + withheld(p, i)); mbar_init(bar(kMKEmpty + i), 1); }
     for (int i = 0; i < C::kSBuffers; ++i) { mbar_init(bar(kMSFull + i), 1); mbar_init(bar(kMSEmpty + i), 4); }
     mbar_init(bar(kMQFull), 4 * C::kGroups);
     mbar_init(bar(kMDrained), 1);
     for (int i = 0; i < C::kRing; ++i) { mbar_init(bar(kMRingFull + i), 1); mbar_init(bar(kMRingEmpty + i), 4); }
     wait->abort = 0;
-    wait->limit_ns = kWaitLimitNs;
+    wait->limit_ns = p.wait_limit_ns;
     mbar_init_fence();
   }
   if (tid < 16) reinterpret_cast<float*>(sm + C::kOffLevels)[tid] = tid < (p.k_bits == 4 ? 16 : 4) ? __ldg(p.cb_k + tid) : 0.f;

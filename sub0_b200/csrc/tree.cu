@@ -21,6 +21,9 @@ __device__ int g_tree_status = 0;
 namespace cda {
 
 // ---- host side ----------------------------------------------------------------------------------------------------------
+static unsigned long long g_wait_limit_ns = umma::kWaitLimitNs;   // diagnostic knobs (cda_b200_kv_debug)
+static int g_withhold_first_k = 0;
+
 static int fill_params(AttendParams& p, const char* what, const void* Q, const void* kv_cache, const int32_t* block_table,
                        const int32_t* cu_q, const int32_t* seq_lens, const float* cb_K, const int64_t* tree_mask,
                        const float* slopes, int64_t T, int B, int H_q, int H_kv, int block_size, int bt_stride, int max_q,
@@ -51,6 +54,7 @@ static int fill_params(AttendParams& p, const char* what, const void* Q, const v
   p.num_blocks = static_cast<int>(num_slots / block_size);
   p.max_q = max_q; p.max_n = max_n; p.k_bits = k_bits; p.v_bits = v_bits; p.slot_bytes = slot_bytes;
   p.scale = scale; p.softcap = softcap; p.window = window;
+  p.wait_limit_ns = g_wait_limit_ns; p.withhold = g_withhold_first_k;
   return CDA_OK;
 }
 
@@ -182,6 +186,12 @@ extern "C" int cda_b200_attention_mass(const void* Q, const void* kv_cache, cons
   // the fewest columns that hold a chunk's rows: a block of more costs the tensor cores and the exponentials as many columns,
   // a block of fewer another pass of the K producers over all tiles
   return rows <= 16 ? launch_mass<16>(p, map, st) : rows <= 64 ? launch_mass<64>(p, map, st) : launch_mass<128>(p, map, st);
+}
+
+extern "C" int cda_b200_kv_debug(int wait_limit_us, int withhold_first_k_arrive) {
+  g_wait_limit_ns = wait_limit_us > 0 ? static_cast<unsigned long long>(wait_limit_us) * 1000ull : umma::kWaitLimitNs;
+  g_withhold_first_k = withhold_first_k_arrive ? 1 : 0;
+  return CDA_OK;
 }
 
 namespace cda {

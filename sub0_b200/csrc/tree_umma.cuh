@@ -414,7 +414,8 @@ __device__ __forceinline__ void feed_ring(const AttendParams& p, const CUtensorM
     for (const int end = min(k + 4, f.n), k0 = k; k < end; ++k, ++issued) {
       if (issued % kFeeders != which) continue;
       const int tile = f.tile0 + k, stage = issued % RING, turn = issued / RING;
-      if (turn > 0) alive = wait_for(empty + 8 * stage, (turn - 1) & 1, wait);
+      // (after a wait elsewhere gave up, producers free stages whose copies may still be on the way: no copy may follow those)
+      if (turn > 0) alive = wait_for(empty + 8 * stage, (turn - 1) & 1, wait) && !wait->abort;
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       const int left = f.seq_len - tile * kKeys, groups = min(8, (left + 15) >> 4), n = tile * kKeys + 16 * (lane & 7);
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
   // (the lengths' way from memory is long: what does not need them goes first)
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {                               // counts: warps that arrive, or one commit
-      mbar_init(bar(kKFull + i), 4); mbar_init(bar(kKEmpty + i), 1); mbar_init(bar(kVFull + i), 4);
+      mbar_init(bar(kKFull + i), 4 + withheld(p, i)); mbar_init(bar(kKEmpty + i), 1); mbar_init(bar(kVFull + i), 4);
       mbar_init(bar(kPFull + i), C::kSoftWarps / C::kStreams); mbar_init(bar(kPvDone + i), 1);
     }
     for (int i = 0; i < C::kSBuffers; ++i) { mbar_init(bar(kSFull + i), 1); mbar_init(bar(kSEmpty + i), C::kSoftWarps / C::kStreams); }
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
     mbar_init(bar(kDrained), 2);
     for (int i = 0; i < C::kRing; ++i) { mbar_init(bar(kRingFull + i), 1); mbar_init(bar(kRingEmpty + i), 8); }
     wait->abort = 0;
-    wait->limit_ns = kWaitLimitNs;
+    wait->limit_ns = p.wait_limit_ns;
     mbar_init_fence();
   }
   if (tid < 32) {                                               // code levels: 16 or 4 of K, then of V

@@ -602,3 +602,9 @@ def kv_status() -> int:
 def kv_clear_status() -> None:
     """Clears the bits of :func:`kv_status`.  Synchronises the device."""
     check(lib.cda_b200_kv_clear_status())
+
+
+def kv_debug(wait_limit_us: int = 0, withhold_first_k_arrive: bool = False) -> None:
+    """Diagnostic knobs of the following :func:`tree_attention` and :func:`attention_mass` launches (see
+    ``cda_b200_kv_debug``); call with no arguments to restore the defaults."""
+    check(lib.cda_b200_kv_debug(int(wait_limit_us), 1 if withhold_first_k_arrive else 0))

@@ -138,6 +138,45 @@ def test_query_limits_far_above_the_chunks(max_q):
     check_tree(c, out, lse)
 
 
+@pytest.mark.parametrize("T,group", [(1, 4), (8, 4), (8, 8), (32, 4)])
+def test_waits_that_run_out_end_the_calls_cleanly(T, group):
+    """One signal of CTA 0 is kept back and the limit of the waits cut to 5 ms, in shares of more tiles than a ring has stages: the
+    CTA gives up, what it had to write stays as it was, all else is right, and so is the next call."""
+    from sub0_b200 import ops
+    B, n = 12, 4000
+    c = S.attend_case([n] * B, [T] * B, H_kv=4, group=group, tree=False, seed=T)
+    want, tol = X.tree_bounds(c)
+    z = S.tree_reference(c)[2].float()
+    start = torch.rand(B, 4, n, generator=torch.Generator().manual_seed(1))
+    gain, mtol = S.mass_reference(c, z, start)
+    dev, cb_V, a = [on(c[k]) for k in ("Q", "cache", "block_table", "seq_lens")], on(c["cb_V"]), call_args(c)
+
+    def tree():
+        out = torch.full_like(dev[0], 7.0)
+        ops.tree_attention(*dev, out, cb_V=cb_V, **a)
+        return out
+
+    def mass():
+        got = on(start).clone()
+        ops.attention_mass(*dev, on(z), got, **a)
+        return got
+
+    ops.kv_clear_status()
+    for run, right, bound, before in ((tree, want, tol, torch.full_like(want, 7.0)), (mass, gain, mtol, start.double())):
+        try:
+            ops.kv_debug(wait_limit_us=5000, withhold_first_k_arrive=True)
+            got = run()
+            assert ops.kv_status() == ops.KV_WAIT_GAVE_UP
+        finally:
+            ops.kv_debug()
+            ops.kv_clear_status()
+        g = got.double().cpu()
+        left = g == before
+        assert bool(left.any()) and bool((left | ((g - right).abs() <= bound)).all())
+        assert not bool(left[-1].any())                               # (the last CTAs' work)
+        assert worst(run(), right, bound) <= 1.0 and ops.kv_status() == 0
+
+
 def busy(milliseconds=60):
     torch.cuda._sleep(int(milliseconds * 1.9e6))
 
