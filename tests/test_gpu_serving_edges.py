@@ -246,6 +246,31 @@ def test_prefill_status_waits_for_other_streams():
 
 # ---- selection and compaction -----------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("rows,M,n,budget", [(1, 300000, 300000, 5000), (2, 270001, 269000, 200000), (90, 20000, 19990, 700), (3, 262144, 262144, 1)])
+def test_select_keys_of_rows_that_do_not_fit_on_chip(rows, M, n, budget):
+    """Slices of more than 32768 keys are read again in every pass; with more rows than half the SMs a row keeps few CTAs."""
+    from sub0_b200 import ops
+    gen = torch.Generator().manual_seed(M)
+    lens = [n] + [int(v) for v in torch.randint(n // 2, n, (rows - 1,), generator=gen)]
+    for ties in (False, True):
+        mass = torch.exp(2 * torch.randn(rows, 1, M, generator=gen))
+        mass = (8 * mass).round() if ties else mass
+        keep, new = ops.select_keys(on(mass), on(torch.tensor(lens)), budget, sink=1 if budget > 1 else 0, recent=min(64, budget // 2))
+        order = torch.arange(M)
+        want = torch.full((rows, 1, budget), -1, dtype=torch.int32)
+        for b, m in enumerate(lens):
+            row = mass[b, 0, :m].clone()
+            row[:1 if budget > 1 else 0] = math.inf
+            row[m - min(64, budget // 2):] = math.inf
+            if m > budget:
+                pick = torch.sort(row, descending=True, stable=True).indices[:budget].sort().values
+            else:
+                pick = order[:m]
+            want[b, 0, :pick.numel()] = pick.to(torch.int32)
+        assert torch.equal(keep.cpu(), want) and new.cpu().tolist() == [min(m, budget) for m in lens]
+    assert ops.kv_status() == 0
+
+
 @pytest.mark.parametrize("shared", [False, True])
 def test_compaction_skips_bad_blocks_with_their_weights(shared):
     """Slots whose block, at either end of the move, lies outside the cache stay as they are; a place that no slot came to has the
