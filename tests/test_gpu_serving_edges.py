@@ -128,6 +128,27 @@ def test_keys_that_are_not_finite_reach_the_rows_that_see_them(k_bits, value):
     assert bool(mass[..., ~bad].isfinite().all())
 
 
+@pytest.mark.parametrize("T,group", [(1, 8), (4, 4), (16, 8)])
+def test_mass_gives_away_what_the_rows_have(T, group):
+    """Every row gives away one, up to the roundings of single terms, which average out, and a bias: the tensor cores cut sums off
+    towards zero.  A score of eight steps of 16 products loses on average half a last place (2^-24) of the partial sum in each,
+    and partial sums average at half of the score: 2^-23 |x| at most eight halves of it, 2^-22 |x|, weighted as the rows weigh
+    their keys.  2^-23 is left for what does not average out of some thousand terms."""
+    from sub0_b200 import ops
+    c = S.attend_case([3000, 2500, 2000], [T] * 3, H_kv=4, group=group, tree=False, seed=T)
+    z = S.tree_reference(c)[2].float()
+    mass = torch.zeros(3, 4, 3000, device=DEV)
+    ops.attention_mass(on(c["Q"]), on(c["cache"]), on(c["block_table"]), on(c["seq_lens"]), on(z), mass, **call_args(c))
+    gain, reach = mass.double().sum().item(), 0.0
+    exact = 0.0                                                       # with the log-sum-exp as the call got it, in 32 bits
+    for b in range(3):
+        x, _, _ = S.sequence_scores(c, b)
+        p = torch.nan_to_num(torch.exp(x - z[b * T:(b + 1) * T].double().view(T, 4, group).permute(1, 0, 2)[..., None]))
+        exact += p.sum().item()
+        reach += (p * torch.nan_to_num(x, neginf=0.0).abs()).sum().item()
+    assert abs(gain - exact) <= 2.0 ** -22 * reach + 2.0 ** -23 * exact, f"{(gain - exact) / exact:.2e} of {reach / exact:.2f}"
+
+
 # ---- limits and status ------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("max_q", [1 << 16, 1 << 23])
