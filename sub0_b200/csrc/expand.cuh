@@ -16,7 +16,16 @@ __device__ __forceinline__ uint32_t permute(uint32_t a, uint32_t b, uint32_t sel
 }
 
 // lo[k], hi[k]: the bytes of levels 4k .. 4k + 3 times the key's norm; a 2-bit side uses k = 0 only.
-struct Planes { uint32_t lo[4], hi[4]; };
+struct Planes {
+  uint32_t lo[4], hi[4];
+  // whether any value is infinite or NaN: the five bits of its exponent are ones
+  __device__ __forceinline__ bool any_not_finite() const {
+    uint32_t any = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) any |= (hi[k] & 0x7C7C7C7Cu) + 0x04040404u;
+    return (any & 0x80808080u) != 0;
+  }
+};
 
 __device__ __forceinline__ Planes make_planes(const float* levels, int groups, float norm) {
   Planes t;

@@ -916,13 +916,9 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
       const uint32_t cell = cell0 + stage * kStageBytes;
       const uint2 norms = lds64(cell + norm_at);
       const bool live = key < *reinterpret_cast<volatile int*>(sm + C::kOffBar + kOffValid + 4 * stage);
-      const bool bad = live && row_not_finite(cell + 16 * p.k_bits, p.v_bits, base + C::kOffLevels + 64, __uint_as_float(norms.y));
-      const float norm = !live || (is_v && bad) ? 0.f : __uint_as_float(is_v ? norms.y : norms.x);      // keys past the end: zero rows
-      const expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
-      if (!is_v) {                                                      // (eight tiles deep: read before S of tile i + 4 is written)
-        const uint32_t bad_keys = __ballot_sync(0xffffffffu, bad);
-        if (lane == 0) *reinterpret_cast<uint32_t*>(sm + C::kOffBad + 16 * (i & 7) + 4 * (warp & 3)) = bad_keys;
-      }
+      const float norm = live ? __uint_as_float(is_v ? norms.y : norms.x) : 0.f;        // keys past the end: zero rows
+      expand::Planes t = expand::make_planes(levels, bits == 4 ? 4 : 1, norm);
+      if (is_v && t.any_not_finite() && row_not_finite(cell + code_at, bits, base + C::kOffLevels + 64, norm)) t = expand::Planes{};
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {                                     // 32 coordinates at a time
         uint32_t v[16];
@@ -940,8 +936,14 @@ __global__ void __launch_bounds__(Cfg<NR>::kThreads, 1) tree_attention_kernel(co
           tmem_st16(lanes + buffer * 64 + 16 * c, v);
         }
       }
-      if (is_v) fence_async_smem();
-      else tmem_wait_st();
+      if (is_v) {
+        fence_async_smem();
+      } else {                                                          // (eight tiles deep: read before S of tile i + 4 is written)
+        const bool bad = live && row_not_finite(cell + 16 * p.k_bits, p.v_bits, base + C::kOffLevels + 64, __uint_as_float(norms.y));
+        const uint32_t bad_keys = __ballot_sync(0xffffffffu, bad);
+        if (lane == 0) *reinterpret_cast<uint32_t*>(sm + C::kOffBad + 16 * (i & 7) + 4 * (warp & 3)) = bad_keys;
+        tmem_wait_st();
+      }
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
