@@ -324,7 +324,8 @@ int cda_b200_attention_mass(const void* Q, const void* kv_cache, const int32_t* 
 
 /* Which `budget` keys of every (sequence, KV head) to keep: the first `sink`, the last `recent`, and of the others those with
  * the largest mass, ties to the lower index (NaN ranks as minus infinity).  keep (B, H_kv, budget) int32 in ascending order,
- * -1 behind the end of a sequence of fewer keys; new_lens (B) int32 = min(seq_lens, budget).  sink + recent <= budget.
+ * -1 behind the end of a sequence of fewer keys; new_lens (B) int32 = min(seq_lens, budget).  sink + recent <= budget; budget and
+ * mass_stride at most 2^31 - 2^16.
  *   mass (B, H_kv, mass_stride) fp32; a sequence longer than mass_stride is cut to it and reported (cda_b200_kv_status)
  * No counterpart in the reference. */
 int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, int32_t* keep, int32_t* new_lens, int B, int H_kv,

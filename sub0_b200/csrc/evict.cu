@@ -328,7 +328,8 @@ extern "C" int cda_b200_select_keys(const float* mass, const int32_t* seq_lens, 
                                     int64_t mass_stride, int budget, int sink, int recent, void* stream) {
   if (B < 0 || H_kv <= 0 || mass_stride < 0 || budget <= 0 || sink < 0 || recent < 0) return fail(CDA_ERR_BAD_ARG, "select_keys: negative size or no budget");
   if (static_cast<int64_t>(sink) + recent > budget) return fail(CDA_ERR_BAD_SHAPE, "select_keys: sink %d + recent %d exceed the budget %d", sink, recent, budget);
-  if (mass_stride > 0x7fff0000ll || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "select_keys: too many weights or rows");
+  // (places are 32-bit integers that loops step past the end of a list)
+  if (mass_stride > 0x7fff0000ll || budget > 0x7fff0000 || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "select_keys: too many weights, rows or kept keys");
   if (B == 0) return CDA_OK;
   if (!mass || !seq_lens || !keep || !new_lens) return fail(CDA_ERR_BAD_ARG, "select_keys: null pointer");
   // CTAs of a row: as few as hold a slice of 16384 keys each, since adding up the histograms costs a CTA as much as some 10000
@@ -357,7 +358,7 @@ extern "C" int cda_b200_compact_cache(void* kv_cache, const int32_t* block_table
   if (slot_bytes != 144 && slot_bytes != 112 && slot_bytes != 80) return fail(CDA_ERR_BAD_SHAPE, "compact_cache: slot width %d is none of 144, 112, 80", slot_bytes);
   if (block_size <= 0 || block_size % 16) return fail(CDA_ERR_BAD_SHAPE, "compact_cache: block_size=%d is not a multiple of 16", block_size);
   if (keep_heads != 1 && keep_heads != H_kv) return fail(CDA_ERR_BAD_SHAPE, "compact_cache: keep has %d heads, the cache %d", keep_heads, H_kv);
-  if (num_slots / block_size > 0x7fffffffll || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "compact_cache: too many slots or sequences");
+  if (num_slots / block_size > 0x7fffffffll || K > 0x7fff0000 || static_cast<int64_t>(B) * H_kv > 0x7fffffffll / 8) return fail(CDA_ERR_N_TOO_LARGE, "compact_cache: too many slots, entries or sequences");
   if (B == 0 || (K == 0 && !mass)) return CDA_OK;
   if (!kv_cache || !block_table || !seq_lens || (K > 0 && !keep)) return fail(CDA_ERR_BAD_ARG, "compact_cache: null pointer");
   if (!aligned16(kv_cache)) return fail(CDA_ERR_BAD_ALIGN, "compact_cache: cache must be 16-byte aligned");

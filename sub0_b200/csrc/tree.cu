@@ -38,6 +38,7 @@ static int fill_params(AttendParams& p, const char* what, const void* Q, const v
   if (block_size <= 0 || block_size % 16) return fail(CDA_ERR_BAD_SHAPE, "%s: block_size=%d is not a multiple of 16", what, block_size);
   if (static_cast<int64_t>(bt_stride) * block_size < max_n) return fail(CDA_ERR_BAD_SHAPE, "%s: block table row shorter than max_seq_len", what);
   if (tree_mask && max_q > 64) return fail(CDA_ERR_UNSUPPORTED, "%s: a tree has at most 64 tokens, max_query_len is %d", what, max_q);
+  if (max_n > 0x7fff0000) return fail(CDA_ERR_N_TOO_LARGE, "%s: max_seq_len %d is too large", what, max_n);
   if (num_slots > 0x7fffffffll) return fail(CDA_ERR_N_TOO_LARGE, "%s: too many slots", what);
   // (a row's token is found by a product with 2^32 / group, exact below 2^26 rows)
   if (static_cast<int64_t>(max_q) * (H_q / H_kv) > 1ll << 26) return fail(CDA_ERR_N_TOO_LARGE, "%s: %d new tokens of %d query heads a KV head are too many", what, max_q, H_q / H_kv);

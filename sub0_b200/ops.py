@@ -416,6 +416,14 @@ def _same_device(dev: torch.device, **tensors: Optional[Tensor]) -> None:
             raise ValueError(f"{name} is on {t.device}, the call on {dev}")
 
 
+def _int(v, name: str) -> int:
+    """A C int: what does not fit would reach the library as another number."""
+    v = int(v)
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise ValueError(f"{name}={v} does not fit 32 bits")
+    return v
+
+
 def _launch(dev: torch.device, fn, *args) -> None:
     """The C entry point on the device's current stream, with that device current."""
     if torch._C._cuda_getDevice() == dev.index:
@@ -461,7 +469,8 @@ def _attend_args(Q, kv_cache, block_table, seq_lens, cb_K, k_bits, v_bits, block
     a.slopes = None if alibi_slopes is None else alibi_slopes.contiguous()
     a.cbk, a.kb, a.vb = _cb(cb_K, a.dev), k_bits, v_bits
     s = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    a.head = (T, B, H_q, H_kv, int(block_size), a.bt.shape[1], int(max_query_len), int(max_seq_len), slots, width, k_bits, v_bits)
+    a.head = (T, B, H_q, H_kv, _int(block_size, "block_size"), a.bt.shape[1], _int(max_query_len, "max_query_len"),
+              _int(max_seq_len, "max_seq_len"), slots, width, k_bits, v_bits)
     a.tail = (s, 0.0 if softcap is None else float(softcap), 0 if window is None else min(int(window), 2 ** 31 - 1))
     return a
 
@@ -548,10 +557,11 @@ def select_keys(mass: Tensor, seq_lens: Tensor, budget: int, *, sink: int = 0, r
     sl = _index(seq_lens)
     if sl.numel() != B:
         raise ValueError("seq_lens must have one element per sequence of mass")
-    keep = sl.new_empty((B, H, max(int(budget), 0)))
+    budget, sink, recent = _int(budget, "budget"), _int(sink, "sink"), _int(recent, "recent")
+    keep = sl.new_empty((B, H, max(budget, 0)))
     new_lens = sl.new_empty(B)
     _launch(mass.device, lib.cda_b200_select_keys, mass.data_ptr(), sl.data_ptr(), keep.data_ptr(), new_lens.data_ptr(), B, H, M,
-            int(budget), int(sink), int(recent))
+            budget, sink, recent)
     return keep, new_lens
 
 
@@ -574,7 +584,7 @@ def compact_cache(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, keep:
     if mass is not None and (mass.dtype != torch.float32 or not mass.is_contiguous() or mass.dim() != 3 or mass.shape[:2] != (B, H)):
         raise ValueError("mass must be a contiguous fp32 CUDA tensor (B, H_kv, M)")
     _launch(dev, lib.cda_b200_compact_cache, cache.data_ptr(), bt.data_ptr(), sl.data_ptr(), kp.data_ptr(), _ptr(st), _ptr(mass),
-            0 if mass is None else mass.shape[2], B, H, kp.shape[2], kp.shape[1], int(block_size), bt.shape[1], cache.shape[0],
+            0 if mass is None else mass.shape[2], B, H, kp.shape[2], kp.shape[1], _int(block_size, "block_size"), bt.shape[1], cache.shape[0],
             cache.shape[2])
 
 
