@@ -288,6 +288,8 @@ int cda_b200_prefill_debug(int wait_limit_us, int withhold_first_k_arrive);
  *   x_n   = scale * q.k_n;  softcap > 0: softcap * tanh(x_n / softcap);  then + slope_h * (pos_n - pos_t)
  *   seen  : n < ctx, or n = ctx + j with bit j of tree_mask[t] set (no mask: j <= t); and pos_t - pos_n < window if window > 0
  *   out   = sum_n softmax(x)_n v_n over the keys seen, lse = log sum_n exp(x_n); a row that sees none: zeros, -inf
+ * Places and positions are those of the cache as it stands: after cda_b200_compact_cache has shortened a sequence they count kept
+ * slots, for each KV head its own.  A row of Q must have a norm below 65504 (its rotated coordinates are taken as fp16 terms).
  * A value row with a coordinate that fp16 cannot hold (a norm that is NaN, infinite or too large) makes NaN of the outputs that
  * see its key, and of no others.
  * The position of a context key is its place, that of a new token ctx + depth, its depth being its place in a chain and

@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_keys_kernel(const float
 // destination, so that slots may be moved in place a step at a time: what a step reads lies at or behind the first place
 // it writes, i.e. behind everything that earlier steps wrote.  A cluster of CTAs shares a step: all read, all wait for one
 // another, all write.  A slot is 5 to 9 pieces of 16 bytes, read and written by neighbouring threads.
-// Floor: every moved slot read and written once (128 lists of 4096 of 16k slots: 23 us at copy bandwidth; measured 47 us;
+// Floor: every moved slot read and written once (128 lists of 4096 of 16k slots: 23 us at copy bandwidth; measured 45 us;
 // single cold launches: 52 us with four CTAs an SM, 58 with the two that 122 registers a thread allow, 63 when a step's entries
 // are looked up while the slots of the one before are read).
 constexpr int kCompactThreads = 256, kCompactStep = 256;      // entries of one CTA in a step

@@ -11,7 +11,7 @@
 // A CTA walks an equal share of all (sequence, KV head) segments' tiles; chunks of more than NR rows pass over the share's
 // tiles once per block of NR rows.
 //
-// Measured (4-bit slots, 8 KV heads, 4 query heads each): one token of 32 sequences of 16k keys 160 to 168 us -- the slots' K half
+// Measured (4-bit slots, 8 KV heads, 4 query heads each): one token of 32 sequences of 16k keys 167 us -- the slots' K half
 // and norms are 49 us at copy bandwidth, whole slots 92 us; the integer pipe is busy 76% of the time and DRAM at 3.8 TB/s --
 // the last 64 tokens of two 30k prompts 90 us (128-row blocks, where it is the exponentials and their sums).
 #pragma once

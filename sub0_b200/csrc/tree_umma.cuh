@@ -24,14 +24,15 @@
 // small value row, they are the output.  (With the reference at the maximum, such an output of 1500 keys was off by 2 %.)
 //
 // Both sides' rows are the format's own, fp16(level * norm), from byte permutes of a key's 16 (or 4) values.  (4-bit value rows from
-// a table of fp16 levels, with the norm on the probability, are rounded in another way and 7 us of 138 faster in the batch below.)
+// a table of fp16 levels, with the norm on the probability, are rounded in another way: 138 us against 145 in the batch below, as both
+// stood then.)
 //
-// Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 145 us (slots: 20 us at copy
-// bandwidth); one tree of 32 x 4 rows over 131k keys 213 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 755 us, 364
-// TFLOP/s.  What bounds it: blocks of up to 64 rows wait for the producers -- the V group takes some 4100 cycles a tile, which is
-// the pace; each K group has twice that for every second tile -- while the tensor cores are busy 16% of the time; blocks of 128
-// rows for the softmax (a chain of some 4800 cycles a tile) and for the clock that the power limit leaves.  A new piece costs 12 to
-// 16 us beside its tiles: query rows, references, the way back, in code that has to come out of L2.
+// Measured (4-bit slots, 8 KV heads, pages of 16): 16 trees of 16 tokens x 4 heads over 16k keys 141 us (slots: 20 us at copy
+// bandwidth); one tree of 32 x 4 rows over 131k keys 206 us; 4 trees of 64 x 8 rows over 32k keys, 2-bit values, 718 us, 383
+// TFLOP/s.  What bounds it: blocks of up to 64 rows wait for the producers -- one V group expands every tile, each K group every
+// second one -- while the tensor cores are busy 17% of the time and no pipe more than 55%; blocks of 128 rows for the softmax (a
+// chain of some 4500 cycles a tile) and for the clock that the power limit leaves.  A new piece costs 12 to 16 us beside its
+// tiles: query rows, references, the way back, in code that has to come out of L2.
 #pragma once
 #include "attend.cuh"
 #include "cache_map.cuh"
@@ -73,7 +74,7 @@ struct Cfg {
   // Registers a thread: softmax takes what the others give back.  32 warps start with 64 (16 x 80 + 16 x 48 a lane; with 88 and 40
   // producers have fewer look-ups in flight: 16 trees of 64 rows 143 us against 138); blocks of 128 rows, whose softmax has the
   // longest chain, do with one K group: 28 warps start with 72 (4 trees of 512 rows 705 us; with two K groups, 88 and 40, 763 us;
-  // with 80 and 56 757 us, with 96 and 40 841 us)
+  // with 80 and 56 757 us, with 96 and 40 841 us; all with references at the maximum, 718 us as it stands)
   static constexpr int kRegsSoft = NR == 128 ? 88 : 80, kRegsOther = 48;
   static constexpr int kRegsAll = 32 * (kSoftWarps * kRegsSoft + (kThreads / 32 - kSoftWarps) * kRegsOther);   // may not exceed the launch's
   static constexpr int kRing = NR == 128 ? 2 : 4;

@@ -571,7 +571,8 @@ def compact_cache(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, keep:
     ``start``).  ``keep`` (B, H_kv or 1, K) int32; every entry satisfies ``start[b] + i <= keep < seq_lens[b]`` or is negative,
     which leaves its destination as it is.  After :func:`select_keys` this shortens the sequences to its ``new_lens``; with
     ``start`` = the context's length and ``keep`` = the accepted path it moves accepted drafts behind the context.  ``mass``
-    moves along, and becomes 0 where no slot comes to a destination and from ``start + K`` to the sequence's end.  The pages written to must belong to one sequence."""
+    moves along, and becomes 0 where no slot comes to a destination and from ``start + K`` to the sequence's end.  The pages
+    written to must belong to one sequence."""
     _cuda(kv_cache, "kv_cache")
     dev = kv_cache.device
     _same_device(dev, block_table=block_table, seq_lens=seq_lens, keep=keep, start=start, mass=mass)
@@ -591,7 +592,8 @@ def compact_cache(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, keep:
 def evict(kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, mass: Tensor, budget: int, *, block_size: int, sink: int = 0,
           recent: int = 0):
     """:func:`select_keys` and :func:`compact_cache` in one call: shortens every sequence to its ``budget`` most attended keys
-    per KV head.  Returns ``keep`` (which token each remaining slot held) and the sequences' new lengths."""
+    per KV head.  Returns ``keep`` (which token each remaining slot held) and the sequences' new lengths.  From then on ``window``
+    and ``alibi_slopes`` of :func:`tree_attention` and :func:`attention_mass` measure kept slots, not tokens."""
     keep, new_lens = select_keys(mass, seq_lens, budget, sink=sink, recent=recent)
     compact_cache(kv_cache, block_table, seq_lens, keep, block_size=block_size, mass=mass)
     return keep, new_lens
